@@ -310,6 +310,61 @@ int mq_swiglu(const void* GU, long ldg, int n, int I, int dtype, void* out, long
  * projection's outputs, n x I each (ldg, ldu) -- two matrices or the two halves of one stacked GEMM output. */
 int mq_swiglu_packed(const void* G, long ldg, const void* U, long ldu, int n, int I, int dtype, void* out, void* stream);
 
+/* ---- (5) tokens to experts and back ---------------------------------------------------------------------------
+ * The reference leaves routing to the model's remote code (quant.py:280-281 runs the block).
+ * Router: scores s = softmax(l) or sigmoid(l) of a token's E logits; experts are ranked by c = s + bias, without a bias by
+ * their logits (the same order).  With n_group > 1 the E experts are n_group runs of equal length: a run counts the sum of
+ * its group_top (1 or 2) best c and only the topk_group best runs stay.  The top_k best remaining experts are taken, best
+ * first, ties (of runs too) to the lowest index; the choice is what 64-bit scores give.  weight = s, divided by the sum
+ * over the chosen (+ 1e-20) if renormalize, times scale.
+ *   logits : T x E (ldl) of type dtype; bias : E fp32, nullable; weights : T x top_k fp32; ids : T x top_k int64.
+ *   score : 0 softmax, 1 sigmoid.  E <= 1024, top_k <= 64, n_group <= 64, top_k <= topk_group * E / n_group.
+ *   A NaN logit or bias counts as -inf; a row of -inf scores 0 (weights 0, ids still valid and distinct). */
+int mq_route_experts(const void* logits, int dtype, long ldl, int T, int E, int top_k, int score, const float* bias,
+                     int n_group, int topk_group, int group_top, int renormalize, float scale, float* weights, long* ids,
+                     void* stream);
+
+/* Stable sort of the n = T * top_k choices in ids by expert: rows[i] = token of the i-th choice in expert order,
+ * offsets[e] .. offsets[e + 1] = the range of expert e (E + 1 values), slots[t, j] (nullable) = position of choice (t, j)
+ * in that order.  Ids outside [0, E) go behind the last expert's range, in order, with slot -1.  Every position of
+ * rows, offsets and slots is written.  E <= 1024, n < 2^31 - 8192.
+ *   workspace: mq_sort_by_expert_workspace_bytes(T, top_k, E) bytes, 4-byte aligned (0: none needed). */
+size_t mq_sort_by_expert_workspace_bytes(int T, int top_k, int E);
+int mq_sort_by_expert(const long* ids, int T, int top_k, int E, long* rows, long* offsets, int* slots, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* out[t, :] = sum_j weights[t, j] * Y[slots[t, j], :], summed in fp32 in the order of j and rounded once; slots outside
+ * [0, S) add nothing.  Y : S x C (ldy), out : T x C (ldo), both of type dtype; out must not overlap Y. */
+int mq_combine_experts(const void* Y, int dtype, long ldy, int S, int C, const int* slots, const float* weights, int T, int k,
+                       void* out, long ldo, void* stream);
+
+/* ---- (6) products on 8-bit integers ----------------------------------------------------------------------------
+ * Runs what GPTQ with 8 bits and one group per row yields (src/gptq.py:156-218: codes minus zero point, one scale per
+ * output channel).
+ * Tokens: scale[r] = max|X[r, :]| / 127 and Q[r, c] = 127 X[r, c] / max|X[r, :]| rounded to the nearest whole number, ties
+ * to even, exactly.  A row of zeros gets scale 0; a row with a NaN or an infinity gets scale NaN and codes 0, so its
+ * products are NaN.  X : n x C (ldx) of type dtype, Q : n x C (ldq). */
+int mq_quantize_tokens(const void* X, int dtype, long ldx, int n, int C, int8_t* Q, long ldq, float* scale, void* stream);
+
+/* Y[m, n] = (sum_k A[m, k] * B[n, k]) * a_scale[m] * b_scale[n] + bias[n]: the sum in 32-bit integers (exact), the rest in
+ * fp32, rounded once to out_dtype.  A : M x K (lda), B : N x K (ldb), Y : M x N (ldy), bias (nullable) : N values of
+ * out_dtype.  swiglu != 0: B holds 2 N rows (N gate rows, then N up rows; b_scale 2 N values, no bias) and
+ * Y[m, n] = silu(gate) * up, rounded once.  K <= 131071.  Any alignment; 16-byte aligned rows (pointers and pitches of
+ * A and B multiples of 16) run fastest.
+ *   workspace: mq_matmul_int8_workspace_bytes(M, N, K, swiglu) bytes, 16-byte aligned (0: none needed). */
+size_t mq_matmul_int8_workspace_bytes(int M, int N, int K, int swiglu);
+int mq_matmul_int8(const int8_t* A, long lda, const float* a_scale, const int8_t* B, long ldb, const float* b_scale,
+                   const void* bias, void* Y, long ldy, int out_dtype, int M, int N, int K, int swiglu, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/* The same with weights per run of rows: rows offsets[e] .. offsets[e + 1) - 1 of Y (device array of E + 1 values, clamped
+ * to [0, S]) are products with B + e * strideB, b_scale + e * N (swiglu: e * 2 N).  Row m of Y takes row rows[m] of A and
+ * a_scale (rows : S int64 on the device; a value outside [0, src_rows) stands for a row of zeros) or, rows == NULL, row
+ * m.  Rows of Y outside every range are left as they are.  E <= 1024. */
+int mq_matmul_int8_grouped(const int8_t* A, long lda, const float* a_scale, int src_rows, const long* rows, int S,
+                           const int8_t* B, long ldb, long strideB, const float* b_scale, int E, const long* offsets, void* Y,
+                           long ldy, int out_dtype, int N, int K, int swiglu, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

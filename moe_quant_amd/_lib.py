@@ -53,6 +53,14 @@ SIGNATURES = {
     "mq_dequant_fp8_block": (_i, [_vp, _l, _i, _i, _vp, _l, _i, _vp, _l, _vp]),
     "mq_swiglu": (_i, [_vp, _l, _i, _i, _i, _vp, _l, _vp]),
     "mq_swiglu_packed": (_i, [_vp, _l, _vp, _l, _i, _i, _i, _vp, _vp]),
+    "mq_route_experts": (_i, [_vp, _i, _l, _i, _i, _i, _i, _vp, _i, _i, _i, _i, _f, _vp, _vp, _vp]),
+    "mq_sort_by_expert_workspace_bytes": (_sz, [_i, _i, _i]),
+    "mq_sort_by_expert": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "mq_combine_experts": (_i, [_vp, _i, _l, _i, _i, _vp, _vp, _i, _i, _vp, _l, _vp]),
+    "mq_quantize_tokens": (_i, [_vp, _i, _l, _i, _i, _vp, _l, _vp, _vp]),
+    "mq_matmul_int8_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "mq_matmul_int8": (_i, [_vp, _l, _vp, _vp, _l, _vp, _vp, _vp, _l, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "mq_matmul_int8_grouped": (_i, [_vp, _l, _vp, _i, _vp, _i, _vp, _l, _l, _vp, _i, _vp, _vp, _l, _i, _i, _i, _i, _vp]),
     "mq_gemm_f32": (_i, [_vp, _l, _l, _vp, _l, _l, _vp, _l, _i, _i, _i, _f, _f, _i, _i, _vp]),
 }
 

@@ -1,0 +1,399 @@
+// Tokens to experts and back: the router's choice, the stable sort of tokens by expert, the weighted sum of the
+// experts' outputs.
+//
+//   mq_route_experts   : logits -> the top_k experts of each token and their weights
+//   mq_sort_by_expert  : expert ids -> token rows in expert order, offsets, and each choice's position in that order
+//   mq_combine_experts : out[t] = sum_j weight[t, j] * Y[slot[t, j]]
+#include <math.h>
+
+#include "common.hpp"
+
+namespace {
+
+enum { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2 };
+enum { SCORE_SOFTMAX = 0, SCORE_SIGMOID = 1 };
+constexpr int ROUTE_MAX_E = 1024;
+
+template <int DT>
+__device__ __forceinline__ float load_val(const void* p, long i) {
+  if (DT == DT_F32) return reinterpret_cast<const float*>(p)[i];
+  if (DT == DT_BF16) return bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(p)[i]);
+  return (float)reinterpret_cast<const _Float16*>(p)[i];
+}
+
+struct RouteArgs {
+  const void* logits;
+  long ldl;
+  int T, E, top_k, score;
+  const float* bias;
+  int n_group, topk_group, group_top, renorm;
+  float scale;
+  float* weights;
+  long* ids;
+};
+
+__device__ __forceinline__ double wave_max(double v) {
+  for (int o = 32; o; o >>= 1) v = fmax(v, __shfl_xor(v, o));
+  return v;
+}
+__device__ __forceinline__ double wave_sum(double v) {
+  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+// One wavefront routes one row, everything in 64 bits (which of two neighbouring experts is chosen hangs on differences
+// far below a 32-bit step).  Lane l holds experts l, l + 64, ...; `group` (LDS, one wavefront's) holds the groups' scores.
+// NaN logits count as -inf (the expert is chosen last); an expert that is equal to the row's maximum has weight exp(0)
+// even where the maximum is +inf; a row whose logits are all -inf scores 0 everywhere.
+template <int DT, int V>
+__device__ __forceinline__ void route_row(const RouteArgs& a, long row, double* group) {
+  const int lane = threadIdx.x & 63;
+  const long base = row * a.ldl;
+  float l[V];
+  double s[V], c[V];
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = lane + 64 * i;
+    l[i] = e < a.E ? load_val<DT>(a.logits, base + e) : -INFINITY;
+    if (!(l[i] == l[i])) l[i] = -INFINITY;
+    m = fmaxf(m, l[i]);
+  }
+  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    if (a.score == SCORE_SIGMOID) {
+      s[i] = 1.0 / (1.0 + exp(-(double)l[i]));
+    } else {
+      s[i] = m == -INFINITY ? 0.0 : (l[i] == m ? 1.0 : exp((double)l[i] - (double)m));
+      sum += s[i];
+    }
+  }
+  if (a.score == SCORE_SOFTMAX) {
+    sum = wave_sum(sum);
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[i] = sum > 0.0 ? s[i] / sum : 0.0;
+  }
+  // without a bias the order of the scores is the order of the logits, which no rounding has touched
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = lane + 64 * i;
+    if (a.bias) {
+      double b = e < a.E ? (double)a.bias[e] : 0.0;
+      c[i] = b == b ? s[i] + b : -INFINITY;
+    } else {
+      c[i] = a.n_group > 1 ? s[i] : (double)l[i];
+    }
+  }
+  unsigned taken = 0;  // bit i: this lane's expert i is out (taken, in a dropped group, or beyond E)
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (lane + 64 * i >= a.E) taken |= 1u << i;
+  if (a.n_group > 1) {
+    const int per = a.E / a.n_group;
+    for (int g = 0; g < a.n_group; ++g) {
+      double best = -INFINITY, second = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int e = lane + 64 * i;
+        if (e / per == g && e < a.E) {
+          second = fmax(second, fmin(best, c[i]));
+          best = fmax(best, c[i]);
+        }
+      }
+      for (int o = 32; o; o >>= 1) {
+        const double ob = __shfl_xor(best, o), os = __shfl_xor(second, o);
+        second = fmax(fmin(best, ob), fmax(second, os));
+        best = fmax(best, ob);
+      }
+      double total = a.group_top == 2 ? best + second : best;
+      if (total != total) total = best;  // an infinite bias of each sign
+      if (lane == 0) group[g] = total;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int e = lane + 64 * i;
+      if (e < a.E) {
+        const int g = e / per;
+        const double mine = group[g];
+        int ahead = 0;
+        for (int q = 0; q < a.n_group; ++q) ahead += group[q] > mine || (group[q] == mine && q < g);
+        if (ahead >= a.topk_group) taken |= 1u << i;
+        if (!a.bias) c[i] = (double)l[i];
+      }
+    }
+  }
+  double sum_w = 0.0, my_w = 0.0;
+  int my_e = 0;
+  for (int j = 0; j < a.top_k; ++j) {
+    double best = -INFINITY, bs = 0.0;
+    int be = 1 << 30;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int e = lane + 64 * i;
+      if (!(taken >> i & 1) && (c[i] > best || (c[i] == best && e < be))) best = c[i], be = e, bs = s[i];
+    }
+    for (int o = 32; o; o >>= 1) {
+      const double ob = __shfl_xor(best, o), os = __shfl_xor(bs, o);
+      const int oe = __shfl_xor(be, o);
+      if (ob > best || (ob == best && oe < be)) best = ob, be = oe, bs = os;
+    }
+    if ((be & 63) == lane) taken |= 1u << (be >> 6);
+    sum_w += bs;
+    if (lane == j) my_w = bs, my_e = be;
+  }
+  if (lane < a.top_k) {
+    if (a.renorm) my_w /= sum_w + 1e-20;
+    a.ids[row * a.top_k + lane] = my_e;
+    a.weights[row * a.top_k + lane] = (float)(my_w * (double)a.scale);
+  }
+}
+
+template <int DT, int V>
+__global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
+  __shared__ double group[4][64];
+  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row < a.T) route_row<DT, V>(a, row, group[threadIdx.x >> 6]);
+}
+
+template <int DT>
+void route_launch(const RouteArgs& a, hipStream_t st) {
+  const dim3 grid((a.T + 3) / 4), block(256);
+  if (a.E <= 64) hipLaunchKernelGGL((route_kernel<DT, 1>), grid, block, 0, st, a);
+  else if (a.E <= 256) hipLaunchKernelGGL((route_kernel<DT, 4>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((route_kernel<DT, 16>), grid, block, 0, st, a);
+}
+
+// ---- sort by expert -----------------------------------------------------------------------------------
+// Stable counting sort of n = T * top_k choices into E + 1 bins (bin E: ids outside [0, E)).  A workgroup owns a run of
+// SORT_CHUNK choices; `count` holds, bin-major, the number of choices of every (bin, workgroup).
+constexpr int SORT_CHUNK = 8192;
+constexpr int SORT_WAVES = 8;
+constexpr int SORT_MAX_E = 1024;
+
+__device__ __forceinline__ int bin_of(long id, int E) { return id < 0 || id >= E ? E : (int)id; }
+
+__global__ __launch_bounds__(512) void sort_count_kernel(const long* __restrict__ ids, int n, int E, int blocks,
+                                                         int* __restrict__ count) {
+  __shared__ int hist[SORT_MAX_E + 1];
+  for (int b = threadIdx.x; b <= E; b += 512) hist[b] = 0;
+  __syncthreads();
+  const int i0 = blockIdx.x * SORT_CHUNK, i1 = min(n, i0 + SORT_CHUNK);
+  for (int i = i0 + threadIdx.x; i < i1; i += 512) atomicAdd(&hist[bin_of(ids[i], E)], 1);
+  __syncthreads();
+  for (int b = threadIdx.x; b <= E; b += 512) count[(long)b * blocks + blockIdx.x] = hist[b];
+}
+
+// One workgroup per bin: its counts become their exclusive prefix sums, its total goes to total[bin].
+__global__ __launch_bounds__(256) void sort_scan_kernel(int* __restrict__ count, int blocks, int* __restrict__ total) {
+  __shared__ int part[4];
+  int* c = count + (long)blockIdx.x * blocks;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int base = 0;
+  for (int i0 = 0; i0 < blocks; i0 += 256) {
+    const int i = i0 + threadIdx.x;
+    const int v = i < blocks ? c[i] : 0;
+    int s = v;
+    for (int o = 1; o < 64; o <<= 1) {
+      const int u = __shfl_up(s, o);
+      if (lane >= o) s += u;
+    }
+    if (lane == 63) part[wave] = s;
+    __syncthreads();
+    int before = base, all = 0;
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) before += part[w];
+      all += part[w];
+    }
+    if (i < blocks) c[i] = before + s - v;
+    base += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) total[blockIdx.x] = base;
+}
+
+// ALONE: one workgroup does the whole sort (n <= SORT_CHUNK) and counts for itself.
+template <bool ALONE>
+__global__ __launch_bounds__(512) void sort_scatter_kernel(const long* __restrict__ ids, int n, int k, int E, int blocks,
+                                                           const int* __restrict__ count, const int* __restrict__ total,
+                                                           long* __restrict__ rows, long* __restrict__ offsets,
+                                                           int* __restrict__ slots) {
+  __shared__ int pos[SORT_WAVES][SORT_MAX_E + 1];  // choices of a bin in a wavefront's run, then its next position
+  __shared__ int start[SORT_MAX_E + 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int w = 0; w < SORT_WAVES; ++w)
+    for (int b = threadIdx.x; b <= E; b += 512) pos[w][b] = 0;
+  __syncthreads();
+  const int per = ALONE ? ((n + SORT_WAVES - 1) / SORT_WAVES + 63) / 64 * 64 : SORT_CHUNK / SORT_WAVES;
+  const long i0 = (long)blockIdx.x * SORT_CHUNK + wave * per;
+  for (int q = 0; q < per; q += 64) {
+    const long i = i0 + q + lane;
+    if (i < n) atomicAdd(&pos[wave][bin_of(ids[i], E)], 1);
+  }
+  __syncthreads();
+  if (wave == 0) {  // exclusive prefix of the bins' totals
+    int base = 0;
+    for (int b0 = 0; b0 <= E; b0 += 64) {
+      const int b = b0 + lane;
+      int v = 0;
+      if (b <= E) {
+        if (ALONE)
+          for (int w = 0; w < SORT_WAVES; ++w) v += pos[w][b];
+        else v = total[b];
+      }
+      int s = v;
+      for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(s, o);
+        if (lane >= o) s += u;
+      }
+      if (b <= E) start[b] = base + s - v;
+      base += __shfl(s, 63);
+    }
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b <= E; b += 512) {
+    int at = start[b] + (ALONE ? 0 : count[(long)b * blocks + blockIdx.x]);
+    if (blockIdx.x == 0) offsets[b] = start[b];
+    for (int w = 0; w < SORT_WAVES; ++w) {
+      const int c = pos[w][b];
+      pos[w][b] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+  for (int q = 0; q < per; q += 64) {
+    const long i = i0 + q + lane;
+    const bool in = i < n;
+    const int b = in ? bin_of(ids[i], E) : E + 1;
+    unsigned long same = ~0ul;  // lanes with this lane's bin
+    for (int bit = 0; bit < 11; ++bit) {
+      const unsigned long set = __ballot(b >> bit & 1);
+      same &= (b >> bit & 1) ? set : ~set;
+    }
+    const int before = __popcll(same & ((1ul << lane) - 1));
+    if (in) {
+      const int at = pos[wave][b] + before;
+      rows[at] = i / k;
+      if (slots) slots[i] = b == E ? -1 : at;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (in && before == 0) pos[wave][b] += __popcll(same);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+}
+
+// ---- combine --------------------------------------------------------------------------------------------
+// One workgroup per (token, 2048 columns); the sum runs in the order of the token's choices, in 32 bits, and is rounded
+// once.  Slots outside [0, S) add nothing.
+template <int DT, bool VEC>
+__global__ __launch_bounds__(256) void combine_kernel(const void* __restrict__ Y, long ldy, int S, int C,
+                                                      const int* __restrict__ slots, const float* __restrict__ weights, int k,
+                                                      void* __restrict__ out, long ldo) {
+  const long t = blockIdx.x;
+  const int c0 = (blockIdx.y * 256 + threadIdx.x) * 8;
+  if (c0 >= C) return;
+  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < k; ++j) {
+    const int s = slots[t * k + j];
+    const float w = weights[t * k + j];
+    if ((unsigned)s >= (unsigned)S) continue;
+    const long at = (long)s * ldy + c0;
+    float v[8];
+    if (VEC) {
+      if (DT == DT_F32) {
+        *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>((const float*)Y + at);
+        *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>((const float*)Y + at + 4);
+      } else {
+        const uint4 u = *reinterpret_cast<const uint4*>((const uint16_t*)Y + at);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = load_val<DT>(&u, e);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = c0 + e < C ? load_val<DT>(Y, at + e) : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = fmaf(w, v[e], acc[e]);
+  }
+  const long to = t * ldo + c0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (VEC || c0 + e < C) {
+      if (DT == DT_F32) ((float*)out)[to + e] = acc[e];
+      else if (DT == DT_BF16) ((uint16_t*)out)[to + e] = f32_to_bf16_bits(acc[e]);
+      else ((_Float16*)out)[to + e] = (_Float16)acc[e];
+    }
+}
+
+template <int DT>
+void combine_launch(const void* Y, long ldy, int S, int C, const int* slots, const float* weights, int T, int k, void* out,
+                    long ldo, hipStream_t st) {
+  const int per16 = DT == DT_F32 ? 4 : 8;  // elements in 16 bytes
+  const bool vec = C % 8 == 0 && ldy % per16 == 0 && ldo % per16 == 0 && ((uintptr_t)Y & 15) == 0 && ((uintptr_t)out & 15) == 0;
+  const dim3 grid(T, (C + 2047) / 2048);
+  if (vec) hipLaunchKernelGGL((combine_kernel<DT, true>), grid, dim3(256), 0, st, Y, ldy, S, C, slots, weights, k, out, ldo);
+  else hipLaunchKernelGGL((combine_kernel<DT, false>), grid, dim3(256), 0, st, Y, ldy, S, C, slots, weights, k, out, ldo);
+}
+
+}  // namespace
+
+extern "C" int mq_route_experts(const void* logits, int dtype, long ldl, int T, int E, int top_k, int score, const float* bias,
+                                int n_group, int topk_group, int group_top, int renormalize, float scale, float* weights,
+                                long* ids, void* stream) {
+  if (T < 0 || E <= 0 || E > ROUTE_MAX_E || top_k <= 0 || top_k > 64 || top_k > E || ldl < E) return MQ_ERR_ARG;
+  if (score != SCORE_SOFTMAX && score != SCORE_SIGMOID) return MQ_ERR_ARG;
+  if (n_group <= 0 || n_group > 64 || E % n_group || topk_group <= 0 || topk_group > n_group) return MQ_ERR_ARG;
+  if (group_top < 1 || group_top > 2 || group_top > E / n_group || (long)topk_group * (E / n_group) < top_k) return MQ_ERR_ARG;
+  if (dtype != DT_F32 && dtype != DT_BF16 && dtype != DT_F16) return MQ_ERR_ARG;
+  if (T == 0) return MQ_OK;
+  if (!logits || !weights || !ids) return MQ_ERR_ARG;
+  RouteArgs a = {logits, ldl, T, E, top_k, score, bias, n_group, topk_group, group_top, renormalize, scale, weights, ids};
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == DT_F32) route_launch<DT_F32>(a, st);
+  else if (dtype == DT_BF16) route_launch<DT_BF16>(a, st);
+  else route_launch<DT_F16>(a, st);
+  return mq_check_launch();
+}
+
+extern "C" size_t mq_sort_by_expert_workspace_bytes(int T, int top_k, int E) {
+  if (T <= 0 || top_k <= 0 || E <= 0 || E > SORT_MAX_E || (long)T * top_k <= SORT_CHUNK) return 0;
+  const size_t blocks = ((size_t)T * top_k + SORT_CHUNK - 1) / SORT_CHUNK;
+  return (blocks + 1) * (E + 1) * sizeof(int);
+}
+
+extern "C" int mq_sort_by_expert(const long* ids, int T, int top_k, int E, long* rows, long* offsets, int* slots,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
+  if (T < 0 || top_k <= 0 || E <= 0 || E > SORT_MAX_E || (long)T * top_k > 0x7fffffffL - SORT_CHUNK) return MQ_ERR_ARG;
+  if (!offsets || (T > 0 && (!ids || !rows))) return MQ_ERR_ARG;
+  hipStream_t st = (hipStream_t)stream;
+  const int n = T * top_k;
+  if (n <= SORT_CHUNK) {
+    hipLaunchKernelGGL((sort_scatter_kernel<true>), dim3(1), dim3(512), 0, st, ids, n, top_k, E, 1, nullptr, nullptr, rows,
+                       offsets, slots);
+    return mq_check_launch();
+  }
+  if (!workspace || workspace_bytes < mq_sort_by_expert_workspace_bytes(T, top_k, E)) return MQ_ERR_WORKSPACE;
+  const int blocks = (n + SORT_CHUNK - 1) / SORT_CHUNK;
+  int* total = reinterpret_cast<int*>(workspace);
+  int* count = total + E + 1;
+  hipLaunchKernelGGL(sort_count_kernel, dim3(blocks), dim3(512), 0, st, ids, n, E, blocks, count);
+  hipLaunchKernelGGL(sort_scan_kernel, dim3(E + 1), dim3(256), 0, st, count, blocks, total);
+  hipLaunchKernelGGL((sort_scatter_kernel<false>), dim3(blocks), dim3(512), 0, st, ids, n, top_k, E, blocks, count, total,
+                     rows, offsets, slots);
+  return mq_check_launch();
+}
+
+extern "C" int mq_combine_experts(const void* Y, int dtype, long ldy, int S, int C, const int* slots, const float* weights,
+                                  int T, int k, void* out, long ldo, void* stream) {
+  if (S < 0 || C <= 0 || T < 0 || k <= 0 || ldy < C || ldo < C) return MQ_ERR_ARG;
+  if (dtype != DT_F32 && dtype != DT_BF16 && dtype != DT_F16) return MQ_ERR_ARG;
+  if (T == 0) return MQ_OK;
+  if (!slots || !weights || !out || (S > 0 && !Y)) return MQ_ERR_ARG;
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == DT_F32) combine_launch<DT_F32>(Y, ldy, S, C, slots, weights, T, k, out, ldo, st);
+  else if (dtype == DT_BF16) combine_launch<DT_BF16>(Y, ldy, S, C, slots, weights, T, k, out, ldo, st);
+  else combine_launch<DT_F16>(Y, ldy, S, C, slots, weights, T, k, out, ldo, st);
+  return mq_check_launch();
+}

@@ -12,12 +12,12 @@ from __future__ import annotations
 
 import time
 from dataclasses import dataclass, field
-from typing import Dict, List, Optional
+from typing import Dict, List, Optional, Union
 
 import torch
 import torch.nn as nn
 
-from . import ops
+from . import ops, quant_utils
 from .gptq import GPTQ
 
 
@@ -45,6 +45,12 @@ class LayerResult:
 
 def route_tokens(expert_ids: torch.Tensor, n_experts: int):
     """expert_ids (T, top_k) -> (order, offsets): order[offsets[e]:offsets[e+1]] are the token rows of expert e."""
+    if expert_ids.is_cuda and expert_ids.dtype == torch.int64 and n_experts <= 1024:
+        rows, offsets, _ = ops.sort_by_expert(expert_ids, n_experts)
+        offsets = offsets.tolist()
+        if offsets[-1] != rows.numel():
+            raise ValueError(f"expert ids must lie in [0, {n_experts})")
+        return rows, offsets
     flat = expert_ids.reshape(-1)
     order = torch.argsort(flat, stable=True)
     counts = torch.bincount(flat, minlength=n_experts)
@@ -53,10 +59,78 @@ def route_tokens(expert_ids: torch.Tensor, n_experts: int):
     return order // expert_ids.shape[1], offsets.tolist()
 
 
+@dataclass
+class Router:
+    """The gate of an MoE block: weight (E, C), the rest as `ops.route_experts` takes it.  Calling it on tokens (T, C) gives
+    (weights (T, top_k) fp32, ids (T, top_k) int64); the logits are fp32."""
+
+    weight: torch.Tensor
+    top_k: int
+    score: str = "softmax"
+    bias: Optional[torch.Tensor] = None
+    n_group: int = 1
+    topk_group: Optional[int] = None
+    group_top: int = 2
+    renormalize: bool = True
+    scale: float = 1.0
+    rows_per_call: int = 1 << 18  # tokens whose fp32 copies and logits are alive at a time
+
+    @torch.no_grad()
+    def __call__(self, x: torch.Tensor):
+        w = self.weight.float().t()
+        parts = [ops.route_experts(xs.float() @ w, self.top_k, score=self.score, bias=self.bias, n_group=self.n_group,
+                                   topk_group=self.topk_group, group_top=self.group_top, renormalize=self.renormalize,
+                                   scale=self.scale) for xs in x.split(self.rows_per_call)]
+        if len(parts) == 1:
+            return parts[0]
+        return torch.cat([p[0] for p in parts]), torch.cat([p[1] for p in parts])
+
+
+@dataclass
+class Int8Experts:
+    """The SwiGLU experts of a block on 8-bit weights with a scale per output channel."""
+
+    gate_up: torch.Tensor  # (E, 2 I, C) int8: the gate projection's rows, then the up projection's
+    gate_up_scale: torch.Tensor  # (E, 2 I) fp32
+    down: torch.Tensor  # (E, C, I) int8
+    down_scale: torch.Tensor  # (E, C) fp32
+
+    @classmethod
+    def from_quantized(cls, experts) -> "Int8Experts":
+        """`experts`: for every expert its (gate, up, down), each the (qweight, scale, zero) that
+        `GPTQ(..., group_size=None).quantize(bits)` returned."""
+        gu, gus, dn, dns = [], [], [], []
+        for gate, up, down in experts:
+            (g, gs), (u, us), (d, ds) = (quant_utils.int8_weight(*w) for w in (gate, up, down))
+            gu.append(torch.cat([g, u]))
+            gus.append(torch.cat([gs, us]))
+            dn.append(d)
+            dns.append(ds)
+        return cls(torch.stack(gu), torch.stack(gus), torch.stack(dn), torch.stack(dns))
+
+
+@torch.no_grad()
+def experts_forward_int8(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, experts: Int8Experts) -> torch.Tensor:
+    """The expert part of a block's forward on its quantized weights:
+    y[t] = sum_j weights[t, j] * down_e(silu(gate_e(x[t])) * up_e(x[t])), e = ids[t, j].  x (T, C) fp32, bf16 or fp16; ids
+    (T, top_k) int64 and weights (T, top_k) fp32 as a `Router` gives them (ids outside the experts add nothing).  Tokens and
+    the product between the projections, held in x's type, are quantized to 8 bits with a scale per row.  Nothing is read
+    back to the host."""
+    E, C = experts.gate_up.shape[0], experts.gate_up.shape[2]
+    if x.dim() != 2 or x.shape[1] != C or ids.shape != weights.shape or ids.dim() != 2 or ids.shape[0] != x.shape[0]:
+        raise ValueError("x must be (T, C) with the experts' C, ids and weights (T, top_k)")
+    rows, offsets, slots = ops.sort_by_expert(ids, E)
+    codes, scale = ops.quantize_tokens(x)
+    h = ops.matmul_int8_grouped(codes, scale, experts.gate_up, experts.gate_up_scale, offsets, rows, x.dtype, swiglu=True)
+    codes, scale = ops.quantize_tokens(h)
+    y = ops.matmul_int8_grouped(codes, scale, experts.down, experts.down_scale, offsets, None, x.dtype)
+    return ops.combine_experts(y, slots, weights)
+
+
 @torch.no_grad()
 def quantize_moe_layer(
     x: torch.Tensor,
-    expert_ids: torch.Tensor,
+    expert_ids: Union[torch.Tensor, Router],
     experts: List[ExpertWeights],
     bits: int = 4,
     group_size: int = 128,
@@ -69,7 +143,7 @@ def quantize_moe_layer(
     group: int = 8,
     overlap: bool = True,
 ) -> LayerResult:
-    """x (T, C) bf16 on the GPU, expert_ids (T, top_k) int64 on the GPU.
+    """x (T, C) bf16 on the GPU, expert_ids (T, top_k) int64 on the GPU, or the block's `Router`, which then chooses.
 
     `group`, `streams`: one linear is a long chain of dependent launches whose critical path (one-workgroup
     diagonal blocks, 64-row column walks) leaves most of the GPU idle.  Experts are therefore quantized `group` at a
@@ -99,6 +173,8 @@ def quantize_moe_layer(
 
     sync()
     t0 = time.perf_counter()
+    if isinstance(expert_ids, Router):
+        expert_ids = expert_ids(x)[1]
     rows, offsets = route_tokens(expert_ids, E)
     sync()
     res.seconds["route"] = time.perf_counter() - t0

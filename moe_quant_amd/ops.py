@@ -4,6 +4,8 @@ from __future__ import annotations
 
 from typing import Optional, Tuple
 
+from contextlib import nullcontext
+
 import torch
 from torch import Tensor
 
@@ -624,6 +626,216 @@ def swiglu_packed(G: Tensor, U: Tensor) -> PackedTokens:
     check(lib.mq_swiglu_packed(G.data_ptr(), G.stride(0) if n > 1 else I, U.data_ptr(), U.stride(0) if n > 1 else I, n, I,
                                _dt(G.dtype), out.data_ptr(), _stream(G)), "mq_swiglu_packed")
     return PackedTokens(out, n, I, G.dtype)
+
+
+# ---- (5) tokens to experts and back -------------------------------------------------------------------
+_HERE = nullcontext()
+
+
+def _on(*ts: Optional[Tensor]):
+    """Every tensor on one GPU; a context in which that GPU is the current one."""
+    _dev(*ts)
+    dev = ts[0].device
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise ValueError("all tensors must be on one device")
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _rows(X: Tensor) -> Tuple[Tensor, int]:
+    """X (n, C) with unit column stride (a copy if it has none) and its row pitch."""
+    n, C = X.shape
+    if (C > 1 and X.stride(1) != 1) or (n > 1 and X.stride(0) < C):
+        X = X.contiguous()
+    return X, (X.stride(0) if n > 1 else C)
+
+
+_SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+def route_experts(logits: Tensor, top_k: int, *, score: str = "softmax", bias: Optional[Tensor] = None, n_group: int = 1,
+                  topk_group: Optional[int] = None, group_top: int = 2, renormalize: bool = True,
+                  scale: float = 1.0) -> Tuple[Tensor, Tensor]:
+    """The router's choice: logits (T, E) fp32/bf16/fp16 -> (weights (T, top_k) fp32, ids (T, top_k) int64).
+
+    s = softmax or sigmoid of a token's logits; experts are ranked by s + bias (bias: (E,) fp32, moves the choice only, not
+    the weights).  With n_group > 1 the experts form n_group runs of equal length; a run counts the sum of its `group_top`
+    (1 or 2) best and only the `topk_group` best runs stay (None: all).  The top_k best remaining experts come best first,
+    ties to the lowest index.  weight = s, divided by the sum over the chosen if `renormalize`, times `scale`.  A NaN logit
+    counts as -inf; a row of -inf has weights 0."""
+    if logits.dim() != 2 or logits.dtype not in _DT:
+        raise ValueError("logits must be (T, E) fp32, bf16 or fp16")
+    T, E = logits.shape
+    if score not in _SCORES:
+        raise ValueError(f"score must be 'softmax' or 'sigmoid', got {score!r}")
+    if not 1 <= E <= 1024 or not 1 <= top_k <= min(E, 64):
+        raise ValueError("1 <= E <= 1024 and 1 <= top_k <= min(E, 64) are needed")
+    if not 1 <= n_group <= 64 or E % n_group:
+        raise ValueError("n_group must divide the number of experts and be at most 64")
+    topk_group = n_group if topk_group is None else topk_group
+    if n_group == 1:
+        group_top = 1
+    if not 1 <= topk_group <= n_group or topk_group * (E // n_group) < top_k:
+        raise ValueError("topk_group groups must hold at least top_k experts")
+    if group_top not in (1, 2) or group_top > E // n_group:
+        raise ValueError("group_top must be 1 or 2 and no more than a group's experts")
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (E,) or not bias.is_contiguous()):
+        raise ValueError("bias must be a contiguous fp32 vector of one value per expert")
+    with _on(logits, bias):
+        logits, ldl = _rows(logits)
+        weights = torch.empty(T, top_k, dtype=torch.float32, device=logits.device)
+        ids = torch.empty(T, top_k, dtype=torch.int64, device=logits.device)
+        rc = _lib.load().mq_route_experts(
+            logits.data_ptr(), _DT[logits.dtype], ldl, T, E, top_k, _SCORES[score], _p(bias), n_group, topk_group, group_top,
+            int(renormalize), float(scale), weights.data_ptr(), ids.data_ptr(), _stream(logits))
+    check(rc, "mq_route_experts")
+    return weights, ids
+
+
+def sort_by_expert(ids: Tensor, n_experts: int) -> Tuple[Tensor, Tensor, Tensor]:
+    """Stable sort of the choices ids (T, top_k) int64 by expert, on the device and without a host read:
+    (rows (T*top_k,) int64, offsets (n_experts + 1,) int64, slots (T, top_k) int32).  rows[offsets[e]:offsets[e + 1]] are
+    the tokens of expert e, slots[t, j] the position of choice (t, j) among `rows`.  Ids outside [0, n_experts) come
+    behind the last expert's, with slot -1."""
+    if ids.dim() != 2 or ids.dtype != torch.int64 or ids.shape[1] < 1:
+        raise ValueError("ids must be (T, top_k) int64")
+    if not 1 <= n_experts <= 1024:
+        raise ValueError("1 <= n_experts <= 1024 is needed")
+    T, k = ids.shape
+    if T * k >= (1 << 31) - 8192:
+        raise ValueError("fewer than 2^31 - 8192 choices are needed")
+    with _on(ids):
+        ids = ids.contiguous()
+        lib, dev = _lib.load(), ids.device
+        rows = torch.empty(T * k, dtype=torch.int64, device=dev)
+        offsets = torch.empty(n_experts + 1, dtype=torch.int64, device=dev)
+        slots = torch.empty(T, k, dtype=torch.int32, device=dev)
+        # (scratch memory of its own for every call: two captured graphs must not share it)
+        need = lib.mq_sort_by_expert_workspace_bytes(T, k, n_experts)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        rc = lib.mq_sort_by_expert(ids.data_ptr(), T, k, n_experts, rows.data_ptr(), offsets.data_ptr(), slots.data_ptr(),
+                                   _p(ws), need, _stream(ids))
+    check(rc, "mq_sort_by_expert")
+    return rows, offsets, slots
+
+
+def combine_experts(Y: Tensor, slots: Tensor, weights: Tensor) -> Tensor:
+    """out[t] = sum_j weights[t, j] * Y[slots[t, j]]: the experts' outputs Y (S, C) fp32/bf16/fp16 (rows in expert order)
+    back to tokens, out (T, C) of Y's type.  slots (T, k) int32 from `sort_by_expert` (outside [0, S): adds nothing),
+    weights (T, k) fp32.  Summed in fp32 in the order of j, rounded once."""
+    if Y.dim() != 2 or Y.dtype not in _DT or Y.shape[1] < 1:
+        raise ValueError("Y must be (S, C) fp32, bf16 or fp16")
+    if slots.dim() != 2 or slots.dtype != torch.int32 or slots.shape[1] < 1:
+        raise ValueError("slots must be (T, k) int32")
+    if weights.shape != slots.shape or weights.dtype != torch.float32:
+        raise ValueError("weights must be fp32 of the shape of slots")
+    with _on(Y, slots, weights):
+        Y, ldy = _rows(Y)
+        slots, weights = slots.contiguous(), weights.contiguous()
+        (S, C), (T, k) = Y.shape, slots.shape
+        out = torch.empty(T, C, dtype=Y.dtype, device=Y.device)
+        rc = _lib.load().mq_combine_experts(Y.data_ptr(), _DT[Y.dtype], ldy, S, C, slots.data_ptr(), weights.data_ptr(), T, k,
+                                            out.data_ptr(), C, _stream(Y))
+    check(rc, "mq_combine_experts")
+    return out
+
+
+# ---- (6) products on 8-bit integers -------------------------------------------------------------------
+_MAX_K = 131071  # a sum of this many products of two bytes stays inside 32 bits
+
+
+def quantize_tokens(X: Tensor) -> Tuple[Tensor, Tensor]:
+    """X (n, C) fp32/bf16/fp16 -> (codes (n, C) int8, scale (n,) fp32): scale = max|x| / 127 of a row, code = x / scale
+    rounded to the nearest whole number, ties to even, as exact arithmetic gives it.  A row with a NaN or an infinity gets
+    scale NaN (its products are NaN, no other row's)."""
+    if X.dim() != 2 or X.dtype not in _DT or X.shape[1] < 1:
+        raise ValueError("X must be (n, C) fp32, bf16 or fp16")
+    with _on(X):
+        X, ldx = _rows(X)
+        n, C = X.shape
+        Q = torch.empty(n, C, dtype=torch.int8, device=X.device)
+        scale = torch.empty(n, dtype=torch.float32, device=X.device)
+        rc = _lib.load().mq_quantize_tokens(X.data_ptr(), _DT[X.dtype], ldx, n, C, Q.data_ptr(), C, scale.data_ptr(),
+                                            _stream(X))
+    check(rc, "mq_quantize_tokens")
+    return Q, scale
+
+
+def _int8_operands(A, a_scale, B, b_scale, out_dtype, swiglu) -> int:
+    """Checks shared by the products; returns N, the columns of the result."""
+    if A.dim() != 2 or A.dtype != torch.int8:
+        raise ValueError("A must be (M, K) int8")
+    K = A.shape[1]
+    if B.dtype != torch.int8 or B.shape[-1] != K or not 1 <= K <= _MAX_K:
+        raise ValueError(f"B must be int8 with A's K columns, 1 <= K <= {_MAX_K}")
+    if a_scale.dtype != torch.float32 or a_scale.shape != A.shape[:1] or not a_scale.is_contiguous():
+        raise ValueError("a_scale must be a contiguous fp32 vector of one value per row of A")
+    if b_scale.dtype != torch.float32 or b_scale.shape != B.shape[:-1] or not b_scale.is_contiguous():
+        raise ValueError("b_scale must be contiguous fp32, one value per row of B")
+    if out_dtype not in _DT:
+        raise ValueError("out_dtype must be fp32, bf16 or fp16")
+    rows = B.shape[-2]
+    if rows < 1 or (swiglu and rows % 2):
+        raise ValueError("B needs at least one row, and gate and up halves of equal length with swiglu")
+    return rows // 2 if swiglu else rows
+
+
+def matmul_int8(A: Tensor, a_scale: Tensor, B: Tensor, b_scale: Tensor, bias: Optional[Tensor] = None,
+                out_dtype: torch.dtype = torch.bfloat16, swiglu: bool = False) -> Tensor:
+    """Y[m, n] = (sum_k A[m, k] B[n, k]) * a_scale[m] * b_scale[n] (+ bias[n]): A (M, K) int8 tokens, B (N, K) int8 weights,
+    the sum exact, one rounding to out_dtype.  bias: (N,) of out_dtype.  swiglu: B holds the gate rows followed by as
+    many up rows and Y = silu(gate) * up (no bias)."""
+    if B.dim() != 2:
+        raise ValueError("B must be (N, K) int8")
+    N = _int8_operands(A, a_scale, B, b_scale, out_dtype, swiglu)
+    if bias is not None and (swiglu or bias.dtype != out_dtype or bias.shape != (N,) or not bias.is_contiguous()):
+        raise ValueError("bias must be a contiguous vector of out_dtype with one value per row of B, and none with swiglu")
+    with _on(A, a_scale, B, b_scale, bias):
+        (A, lda), (B, ldb) = _rows(A), _rows(B)
+        M, K = A.shape
+        lib = _lib.load()
+        Y = torch.empty(M, N, dtype=out_dtype, device=A.device)
+        need = lib.mq_matmul_int8_workspace_bytes(M, N, K, int(swiglu))
+        ws = torch.empty(need, dtype=torch.uint8, device=A.device) if need else None
+        rc = lib.mq_matmul_int8(A.data_ptr(), lda, a_scale.data_ptr(), B.data_ptr(), ldb, b_scale.data_ptr(), _p(bias),
+                                Y.data_ptr(), N, _DT[out_dtype], M, N, K, int(swiglu), _p(ws), need, _stream(A))
+    check(rc, "mq_matmul_int8")
+    return Y
+
+
+def matmul_int8_grouped(A: Tensor, a_scale: Tensor, B: Tensor, b_scale: Tensor, offsets: Tensor,
+                        rows: Optional[Tensor] = None, out_dtype: torch.dtype = torch.bfloat16, swiglu: bool = False,
+                        out: Optional[Tensor] = None) -> Tensor:
+    """`matmul_int8` for the experts of a block in one call: rows offsets[e]:offsets[e + 1] of the result are products with
+    B[e] (B (E, N, K) int8, b_scale (E, N) fp32, offsets (E + 1,) int64 on the device: nothing is read back).  rows (S,)
+    int64: row m of the result takes row rows[m] of A (outside A: a row of zeros); None: row m.  Rows outside every
+    range are left as they are in `out` (S, N), and undefined without one."""
+    if B.dim() != 3:
+        raise ValueError("B must be (E, N, K) int8")
+    N = _int8_operands(A, a_scale, B, b_scale, out_dtype, swiglu)
+    E = B.shape[0]
+    if not 1 <= E <= 1024:
+        raise ValueError("1 to 1024 experts are needed")
+    if offsets.dtype != torch.int64 or offsets.shape != (E + 1,) or not offsets.is_contiguous():
+        raise ValueError("offsets must be a contiguous int64 vector of E + 1 values")
+    if rows is not None and (rows.dtype != torch.int64 or rows.dim() != 1 or not rows.is_contiguous()):
+        raise ValueError("rows must be a contiguous int64 vector")
+    S = A.shape[0] if rows is None else rows.numel()
+    if out is not None and (out.shape != (S, N) or out.dtype != out_dtype or (N > 1 and out.stride(1) != 1)
+                            or (S > 1 and out.stride(0) < N)):
+        raise ValueError("out must be (S, N) of out_dtype with unit column stride")
+    with _on(A, a_scale, B, b_scale, offsets, rows, out):
+        A, lda = _rows(A)
+        if B.stride(2) != 1 or B.stride(1) < B.shape[2] or B.stride(0) < 0:
+            B = B.contiguous()
+        if out is None:
+            out = torch.empty(S, N, dtype=out_dtype, device=A.device)
+        rc = _lib.load().mq_matmul_int8_grouped(
+            A.data_ptr(), lda, a_scale.data_ptr(), A.shape[0], _p(rows), S, B.data_ptr(), B.stride(1), B.stride(0),
+            b_scale.data_ptr(), E, offsets.data_ptr(), out.data_ptr(), out.stride(0) if S > 1 else N, _DT[out_dtype], N,
+            A.shape[1], int(swiglu), _stream(A))
+    check(rc, "mq_matmul_int8_grouped")
+    return out
 
 
 def gemm_f32_(A, sam, sak, B, sbk, sbn, Cm, M, N, K, alpha=1.0, beta=0.0, tri=0, ktrim=0):

@@ -108,6 +108,29 @@ def dequantize_linear_weight(qweight: Tensor, scale: Tensor, zero: Tensor, perm:
     return weight
 
 
+def int8_weight(qweight: Tensor, scale: Tensor, zero: Tensor):
+    """What `GPTQ(..., group_size=None).quantize(bits)` returns, 2 to 8 bits with one scale per row, as the operands of the
+    8-bit products: (codes minus zero point (R, C) int8, scale (R,) fp32)."""
+    if qweight.dtype != torch.uint8 or qweight.dim() != 2:
+        raise ValueError("qweight must be (R, C) uint8")
+    R = qweight.shape[0]
+    if scale.numel() != R or zero.numel() != R:
+        raise ValueError("the 8-bit products take one scale per row: quantize with group_size=None")
+    shifted = qweight.to(torch.int16) - zero.reshape(R, 1).to(torch.int16)
+    if R and shifted.numel() and (int(shifted.min()) < -128 or int(shifted.max()) > 127):
+        raise ValueError("codes minus zero point must fit 8 bits")
+    return shifted.to(torch.int8), scale.reshape(R).to(torch.float32)
+
+
+def linear_int8(x: Tensor, weight: Tensor, weight_scale: Tensor, bias: Optional[Tensor] = None) -> Tensor:
+    """x (..., C) fp32, bf16 or fp16 through a linear layer on 8-bit weights (R, C) with a scale per row (`int8_weight`);
+    every token is quantized to 8 bits with a scale of its own on the way in.  Returns (..., R) of x's type."""
+    if x.dim() < 1:
+        raise ValueError("x must be (..., C)")
+    codes, scale = ops.quantize_tokens(x.reshape(-1, x.shape[-1]))
+    return ops.matmul_int8(codes, scale, weight, weight_scale, bias, x.dtype).view(*x.shape[:-1], weight.shape[0])
+
+
 def get_relative_mse_error(q: Tensor, w: Tensor, H: Optional[Tensor] = None):
     """src/quant_utils.py:259-264."""
     delta = q - w
