@@ -5,7 +5,7 @@
 //   mq_matmul_int8_grouped : the same, every run of rows with the weights of its expert
 #include <math.h>
 
-#include <mutex>
+#include <atomic>
 
 #include "common.hpp"
 
@@ -29,50 +29,146 @@ __device__ __forceinline__ void store_val(void* p, long i, float v) {
 }
 
 // ---- quantize ---------------------------------------------------------------------------------------------
-// The nearest whole number to 127 x / top, ties to even, as exact arithmetic gives it: x * inv (inv = 127 / top, 32 bits)
-// is within 2^-14 of the quotient, so it decides except next to a border m + 1/2; there 254 |x| and (2 m + 1) top, both
+// The nearest whole number to 127 x / top, ties to even, as exact arithmetic gives it: z = x * (127 / top) in 32 bits is
+// within 2^-14 of the quotient, so rounding z decides except next to a border m + 1/2; there 254 |x| and (2 m + 1) top, both
 // exact in 64 bits, are compared.
-__device__ __forceinline__ int code_of(float x, float top, float inv) {
-  const float z = fabsf(x * inv);
-  float m = floorf(z);
-  const float part = z - m;
-  float r;
-  if (fabsf(part - 0.5f) < 1.220703125e-4f) {
-    const double have = 254.0 * (double)fabsf(x), border = (2.0 * (double)m + 1.0) * (double)top;
-    const bool odd = ((int)m) & 1;
-    r = m + ((have > border || (have == border && odd)) ? 1.f : 0.f);
-  } else {
-    r = m + (part > 0.5f ? 1.f : 0.f);
-  }
-  const int q = (int)r;
-  return x < 0.f ? -q : q;
+__device__ __forceinline__ int exact_code(float x, float top, float inv) {
+  const float m = floorf(fabsf(x * inv) - 0.25f);  // next to a border m + 1/2: its m
+  const double have = 254.0 * (double)fabsf(x), border = (2.0 * (double)m + 1.0) * (double)top;
+  const int r = (int)m + (have > border || (have == border && ((int)m & 1)) ? 1 : 0);
+  return x < 0.f ? -r : r;
 }
 
-// One workgroup per token: the largest magnitude, then the codes (the second read of the row comes from the cache).  A row
-// that holds a NaN or an infinity gets scale NaN and codes 0: its products are NaN, no other token's are.
+// eight codes as bytes.  z + 1.5 * 2^23 rounds z to a whole number, ties to even, and ends in its two's complement.
+__device__ __forceinline__ uint2 eight_codes(const float* x, float top, float inv) {
+  uint32_t t[8];
+  float worst = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float z = x[i] * inv, s = z + 12582912.f;
+    t[i] = __float_as_uint(s);
+    worst = fmaxf(worst, fabsf(z - (s - 12582912.f)));
+  }
+  if (worst > 0.5f - 1.220703125e-4f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float z = x[i] * inv;
+      if (fabsf(z - (__uint_as_float(t[i]) - 12582912.f)) > 0.5f - 1.220703125e-4f) t[i] = (uint32_t)exact_code(x[i], top, inv);
+    }
+  }
+  uint2 out;
+  out.x = __builtin_amdgcn_perm(t[3], t[2], 0x0c0c0400u) << 16 | __builtin_amdgcn_perm(t[1], t[0], 0x0c0c0400u);
+  out.y = __builtin_amdgcn_perm(t[7], t[6], 0x0c0c0400u) << 16 | __builtin_amdgcn_perm(t[5], t[4], 0x0c0c0400u);
+  return out;
+}
+
+// elements c .. c + 7 of a row of C, zeros beyond its end (any alignment)
 template <int DT>
-__global__ __launch_bounds__(256) void quantize_tokens_kernel(const void* __restrict__ X, long ldx, int C,
+__device__ __forceinline__ void load8(const void* row, int c, int C, float* x) {
+  if (c + 8 <= C) {
+    if (DT == DT_F32) {
+      __builtin_memcpy(x, (const float*)row + c, 32);
+    } else {
+      uint16_t h[8];
+      __builtin_memcpy(h, (const uint16_t*)row + c, 16);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = load_val<DT>(h, i);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = c + i < C ? load_val<DT>(row, c + i) : 0.f;
+  }
+}
+
+// TPR threads per token, eight values each in turn: the largest magnitude first, then the codes, from the NV vectors a
+// thread keeps in registers (NV = 0: rows too long for that, read twice, the second time from the cache).  A row that holds
+// a NaN or an infinity gets scale NaN and codes 0: its products are NaN, no other token's are.
+template <int DT, int TPR, int NV>
+__global__ __launch_bounds__(256) void quantize_tokens_kernel(const void* __restrict__ X, long ldx, int n, int C,
                                                               int8_t* __restrict__ Q, long ldq, float* __restrict__ scale) {
   __shared__ float part[4];
-  const long row = blockIdx.x;
+  constexpr int KEEP = NV ? NV : 1;
+  const int t = threadIdx.x % TPR;
+  const long row = (long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  if (TPR < 256 && row >= n) return;
+  const void* x0 = (const char*)X + row * ldx * (DT == DT_F32 ? 4 : 2);
+  float x[KEEP][8];
   float top = 0.f;
   bool bad = false;
-  for (int c = threadIdx.x; c < C; c += 256) {
-    const float v = fabsf(load_val<DT>(X, row * ldx + c));
-    bad |= !(v <= 3.402823466e38f);
-    top = fmaxf(top, v);
+  auto look = [&](const float* v) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      bad |= v[i] != v[i];
+      top = fmaxf(top, fabsf(v[i]));
+    }
+  };
+  if (NV) {
+#pragma unroll
+    for (int v = 0; v < KEEP; ++v) load8<DT>(x0, (v * TPR + t) * 8, C, x[v]);
+#pragma unroll
+    for (int v = 0; v < KEEP; ++v) look(x[v]);
+  } else {
+    for (int c = 8 * t; c < C; c += 8 * TPR) {
+      load8<DT>(x0, c, C, x[0]);
+      look(x[0]);
+    }
   }
   if (bad) top = INFINITY;
   for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+  if (TPR == 256) {
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+  }
   const bool fine = top <= 3.402823466e38f;
-  if (threadIdx.x == 0) scale[row] = fine ? top / 127.f : NAN;
+  if (t == 0) scale[row] = fine ? top / 127.f : NAN;
   const bool zero = !fine || top == 0.f;
   const float up = top < 0x1p-90f ? 0x1p90f : 1.f;  // keeps 127 / top finite; exact
-  for (int c = threadIdx.x; c < C; c += 256)
-    Q[row * ldq + c] = zero ? 0 : (int8_t)code_of(load_val<DT>(X, row * ldx + c) * up, top * up, 127.f / (top * up));
+  top *= up;
+  const float inv = zero ? 0.f : 127.f / top;
+  int8_t* q = Q + row * ldq;
+  auto put = [&](float* v, int c) {
+    if (c >= C) return;
+    if (zero || up != 1.f) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = zero ? 0.f : v[i] * up;
+    }
+    const uint2 w = eight_codes(v, top, inv);
+    if (c + 8 <= C) {
+      __builtin_memcpy(q + c, &w, 8);
+    } else {
+      int8_t b[8];
+      __builtin_memcpy(b, &w, 8);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c + i < C) q[c + i] = b[i];
+    }
+  };
+  if (NV) {
+#pragma unroll
+    for (int v = 0; v < KEEP; ++v) put(x[v], (v * TPR + t) * 8);
+  } else {
+    for (int c = 8 * t; c < C; c += 8 * TPR) {
+      load8<DT>(x0, c, C, x[0]);
+      put(x[0], c);
+    }
+  }
+}
+
+template <int DT>
+void quantize_launch(const void* X, long ldx, int n, int C, int8_t* Q, long ldq, float* scale, hipStream_t st) {
+#define MQ_QUANT(TPR, NV)                                                                                            \
+  hipLaunchKernelGGL((quantize_tokens_kernel<DT, TPR, NV>), dim3((n + 256 / TPR - 1) / (256 / TPR)), dim3(256), 0, st, X, \
+                     ldx, n, C, Q, ldq, scale)
+  if (C <= 512) MQ_QUANT(64, 1);
+  else if (C <= 1024) MQ_QUANT(64, 2);
+  else if (C <= 2048) MQ_QUANT(256, 1);
+  else if (C <= 4096) MQ_QUANT(256, 2);
+  else if (C <= 8192) MQ_QUANT(256, 4);
+  else if (C <= 16384) MQ_QUANT(256, 8);
+  else if (C <= 24576) MQ_QUANT(256, 12);
+  else MQ_QUANT(256, 0);
+#undef MQ_QUANT
 }
 
 // ---- product ------------------------------------------------------------------------------------------------
@@ -94,37 +190,59 @@ struct Int8Args {
   int vec_out;
 };
 
-// Which rows a workgroup's row tile covers: its tile index -> expert, first row, end.  Experts' tiles follow one another;
-// every wavefront finds its own with a prefix sum over the experts, 64 at a time.  Offsets are clamped to [0, M].
-__device__ __forceinline__ bool find_tile(const Int8Args& a, int tile, int bm, int& e_out, int& m0, int& mend) {
-  const int lane = threadIdx.x & 63;
-  int base = 0;
-  for (int e0 = 0; e0 < a.E; e0 += 64) {
-    const int e = e0 + lane;
-    int lo = 0, hi = 0;
-    if (e < a.E) {
-      lo = (int)min(max(a.offsets[e], 0l), (long)a.M);
-      hi = (int)min(max(a.offsets[e + 1], (long)lo), (long)a.M);
+// Row tiles of a grouped product: the experts' tiles of bm rows follow one another.  `locate` finds the workgroup's own:
+// a lane counts the tiles of E / 64 consecutive experts, a prefix sum over the lanes gives the number of tiles in all and
+// the lane that holds the wanted one.  Offsets are clamped to [0, M].
+struct RowTiles {
+  int first, per;  // this lane's experts
+  int before, total;
+
+  __device__ __forceinline__ static void range(const Int8Args& a, int e, int& lo, int& hi) {
+    lo = (int)min(max(a.offsets[e], 0l), (long)a.M);
+    hi = (int)min(max(a.offsets[e + 1], (long)lo), (long)a.M);
+  }
+  __device__ __forceinline__ void count(const Int8Args& a, int bm) {
+    const int lane = threadIdx.x & 63;
+    per = (a.E + 63) >> 6;
+    first = lane * per;
+    int mine = 0;
+    for (int i = 0; i < per; ++i) {
+      const int e = first + i;
+      if (e < a.E) {
+        int lo, hi;
+        range(a, e, lo, hi);
+        mine += (hi - lo + bm - 1) / bm;
+      }
     }
-    const int tiles = (hi - lo + bm - 1) / bm;
-    int s = tiles;
+    int s = mine;
     for (int o = 1; o < 64; o <<= 1) {
       const int u = __shfl_up(s, o);
       if (lane >= o) s += u;
     }
-    const bool mine = tile >= base + s - tiles && tile < base + s;
-    const unsigned long who = __ballot(mine);
-    if (who) {
-      const int src = __builtin_ctzll(who);
-      e_out = e0 + src;
-      m0 = __shfl(lo, src) + (tile - __shfl(base + s - tiles, src)) * bm;
-      mend = min(m0 + bm, __shfl(hi, src));
-      return true;
-    }
-    base += __shfl(s, 63);
+    before = s - mine;
+    total = __builtin_amdgcn_readlane(s, 63);
   }
-  return false;
-}
+  // tile < total: its expert and rows m0 .. mend - 1
+  __device__ __forceinline__ void locate(const Int8Args& a, int bm, int tile, int& e_out, int& m0, int& mend) const {
+    const int lane = threadIdx.x & 63;
+    const unsigned long who = __ballot(before <= tile);  // lanes 0 .. the one that holds it
+    const int src = 63 - __builtin_clzll(who);
+    int left = tile - __builtin_amdgcn_readlane(before, src);
+    int e = src * per;
+    for (;; ++e) {
+      int lo, hi;
+      range(a, e, lo, hi);
+      const int tiles = (hi - lo + bm - 1) / bm;
+      if (left < tiles || e + 1 >= a.E) {
+        e_out = e;
+        m0 = lo + left * bm;
+        mend = min(m0 + bm, hi);
+        return;
+      }
+      left -= tiles;
+    }
+  }
+};
 
 // four results of one row, columns n .. n + 3, as far as they exist
 template <int DT>
@@ -173,7 +291,12 @@ __global__ __launch_bounds__(256) void int8_any_kernel(Int8Args a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wm = wave >> 1, wn = wave & 1;
   int e = 0, m0 = blockIdx.y * GBM, mend = min(m0 + GBM, a.M);
-  if (a.offsets && !find_tile(a, blockIdx.y, GBM, e, m0, mend)) return;
+  if (a.offsets) {
+    RowTiles t;
+    t.count(a, GBM);
+    if ((int)blockIdx.y >= t.total) return;
+    t.locate(a, GBM, blockIdx.y, e, m0, mend);
+  }
   constexpr int OUTN = SWIGLU ? GBN / 2 : GBN;
   const int n0 = blockIdx.x * OUTN;
   const int8_t* B = a.B + (long)e * a.strideB;
@@ -264,17 +387,29 @@ __global__ __launch_bounds__(256) void int8_any_kernel(Int8Args a) {
   }
 }
 
-// 256 x 256 tiles for rows of at least 16 bytes that start at multiples of 4: eight wavefronts of 128 x 64, two per SIMD,
-// four stages of 64 bytes of every row in shared memory, filled by direct 16-byte loads.
+// Tiles of 256 x 256 for rows of at least 16 bytes that start at multiples of 4.  One workgroup per CU, eight wavefronts of
+// 128 x 64, takes one tile after the other; four stages of 64 bytes of every row in shared memory (128 KB), filled by
+// direct 16-byte loads.
 //   Layout of a stage: 256 token rows, then 256 weight rows, 64 bytes each; the 16-byte chunk c of row r lies at position
 //   c ^ (r / 4 % 4), so that 16 lanes reading chunk c of 16 rows touch every bank once.
 //   Pipeline: while the matrix instructions of one half of a stage run, the fragments of the other half are read; the loads
-//   of stage t + 4 are issued into the slot of stage t once every wavefront has read its last fragment (one barrier a stage,
-//   waits for exactly the loads that must have landed).
-//   The last stage: a chunk that reaches beyond K is loaded from the last 16 bytes of the row instead (never outside it),
+//   of stage t + 4 are issued into the slot of stage t once every wavefront has read its last fragment (one barrier a
+//   stage, waits for exactly the loads that must have landed).  The stages of the next tile follow those of this one
+//   without a gap, so its first loads are in flight while this tile's results are written.
+//   The end of a row: a chunk that reaches beyond K is loaded from the last 16 bytes of the row instead (never outside it),
 //   and the tokens' fragments drop the bytes that belong to earlier chunks, or all of them.
+//   A wavefront computes only the 32-row blocks (NB of its four) that hold any rows.
 constexpr int TM = 256, TN = 256, TK = 64, NST = 4, STAGE = (TM + TN) * TK;
-constexpr size_t TILE_SMEM = (size_t)NST * STAGE;
+constexpr int MIN_STAGES = 7;  // what the hand-over to the next tile needs; beyond K everything counts as zero
+constexpr int MAX_GROUPS = 1024;
+struct TileShared {
+  int8_t stage[NST][STAGE];
+  long rows[3][TM];            // gathered products: rows of A of the last tile (a slow wavefront may still write it),
+                               // of this one and of the next
+  int full[MAX_GROUPS + 64], part[MAX_GROUPS + 64];  // whole tiles and partly filled ones before expert e
+  int lo[MAX_GROUPS], hi[MAX_GROUPS];
+};
+static_assert(sizeof(TileShared) <= 160 * 1024, "shared memory of a CU");
 
 // lane i copies 16 bytes from its own address to LDS byte lds_addr + 16 i.  (Inline assembly: told about an LDS-writing
 // load, the compiler would drain all of them before the next LDS read.  The kernel orders loads and reads itself.)
@@ -291,153 +426,336 @@ __device__ __forceinline__ intx4 keep_from(intx4 v, int drop) {  // bytes 0 .. d
   return v;
 }
 
+// the same with four bytes a lane
+__device__ __forceinline__ void load_lds4(const void* p, unsigned lds_addr) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(lds_addr) : "memory", "m0");
+}
+
+struct Job {
+  int e, m0, mend, n0;
+};
+
+template <int DT, bool SWIGLU>
+struct TileKernel {
+  static constexpr int OUTN = SWIGLU ? TN / 2 : TN;
+  const Int8Args& a;
+  TileShared& sh;
+  const int lane, wave, wm, wn, lr, lk;
+  const int nk;         // stages of a tile
+  const int chunk;      // this lane's chunk of a stage's 64 bytes in direct loads
+  const unsigned lds0;  // LDS address of the stages
+  const unsigned rows0;
+  intx16 acc[4][2];
+  intx4 fa0[4], fb0[2];
+  const int8_t *src[4], *next[4];
+  int slot;
+
+  __device__ __forceinline__ static unsigned lds_of(const void* p) {
+    return __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p);
+  }
+  __device__ __forceinline__ TileKernel(const Int8Args& args, TileShared& s)
+      : a(args), sh(s), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), wm(wave >> 2),
+        wn(wave & 3), lr(lane & 31), lk(lane >> 5), nk(max((args.K + TK - 1) / TK, MIN_STAGES)),
+        chunk((lane & 3) ^ (lane >> 4)), lds0(lds_of(&s.stage[0][0])), rows0(lds_of(&s.rows[0][0])), slot(0) {}
+
+  // Experts' ranges (clamped to [0, M]; a plain product is one expert's) and the whole and partly filled row tiles before
+  // each; returns how many there are of both.
+  __device__ __forceinline__ int2 table() {
+    for (int e = threadIdx.x; e < a.E; e += 512) {
+      const int lo = a.offsets ? (int)min(max(a.offsets[e], 0l), (long)a.M) : 0;
+      sh.lo[e] = lo;
+      sh.hi[e] = a.offsets ? (int)min(max(a.offsets[e + 1], (long)lo), (long)a.M) : a.M;
+    }
+    __syncthreads();
+    int2 sum = {0, 0};  // every wavefront sums for itself, the first one writes
+    for (int e0 = 0; e0 < a.E; e0 += 64) {
+      const int e = e0 + lane, n = e < a.E ? sh.hi[e] - sh.lo[e] : 0;
+      const int mine_f = n / TM, mine_p = n % TM ? 1 : 0;
+      int f = mine_f, p = mine_p;
+      for (int o = 1; o < 64; o <<= 1) {
+        const int uf = __shfl_up(f, o), up = __shfl_up(p, o);
+        if (lane >= o) f += uf, p += up;
+      }
+      if (wave == 0) {  // (up to 63 entries beyond E, all = the sums)
+        sh.full[e] = sum.x + f - mine_f;
+        sh.part[e] = sum.y + p - mine_p;
+      }
+      sum.x += __builtin_amdgcn_readlane(f, 63);
+      sum.y += __builtin_amdgcn_readlane(p, 63);
+    }
+    __syncthreads();
+    return sum;
+  }
+
+  // the last expert with start[e] <= tile: 64 candidates at once, twice
+  __device__ __forceinline__ int find(const int* start, int tile) const {
+    const int per = (a.E + 63) >> 6;
+    const int p0 = min(lane * per, a.E);
+    const unsigned long w0 = __ballot(p0 < a.E && start[p0] <= tile);
+    const int b0 = (63 - __builtin_clzll(w0)) * per;
+    const unsigned long w1 = __ballot(lane < per && b0 + lane < a.E && start[b0 + lane] <= tile);
+    return __builtin_amdgcn_readfirstlane(b0 + 63 - __builtin_clzll(w1));
+  }
+
+  // job `id` of the whole tiles (in an expert: bands of four row tiles, the rows of a band first, so that what an XCD works
+  // on at a time shares few panels) or of the partly filled ones
+  __device__ __forceinline__ Job job(bool whole, int id) const {
+    const int nt = (a.N + OUTN - 1) / OUTN;
+    const int tile = id / nt;
+    Job j;
+    if (whole) {
+      j.e = find(sh.full, tile);
+      const int in_e = id - sh.full[j.e] * nt, count = (sh.hi[j.e] - sh.lo[j.e]) / TM;
+      const int band = in_e / (4 * nt), in = in_e - band * 4 * nt, rows = min(4, count - 4 * band);
+      j.m0 = sh.lo[j.e] + (4 * band + in % rows) * TM;
+      j.mend = j.m0 + TM;
+      j.n0 = in / rows * OUTN;
+    } else {
+      j.e = find(sh.part, tile);
+      j.mend = sh.hi[j.e];
+      j.m0 = j.mend - (j.mend - sh.lo[j.e]) % TM;
+      j.n0 = (id - tile * nt) * OUTN;
+    }
+    j.m0 = __builtin_amdgcn_readfirstlane(j.m0);
+    j.mend = __builtin_amdgcn_readfirstlane(j.mend);
+    j.n0 = __builtin_amdgcn_readfirstlane(j.n0);
+    return j;
+  }
+
+  // Where this wavefront's direct loads of a tile start: rows 32 wave + 16 q + lane / 4 of the tokens (q = 0, 1) and of the
+  // weights (q = 2, 3)
+  __device__ __forceinline__ void sources(const Job& j, int buf, const int8_t** p) const {
+    const int8_t* B = a.B + (long)j.e * a.strideB;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int r = 32 * wave + 16 * q + (lane >> 2);
+      // SwiGLU: rows 0..31 of every 64 are gate rows, 32..63 the up rows of the same columns
+      int col = SWIGLU ? j.n0 + (r >> 6) * 32 + (r & 31) : j.n0 + r;
+      if (col >= a.N) col = j.n0;
+      p[2 + q] = B + (long)(SWIGLU && (r & 32) ? a.N + col : col) * a.ldb + 16 * chunk;
+      const long from = a.rows ? sh.rows[buf][r] : min(j.m0 + r, j.mend - 1);
+      p[q] = from >= 0 && from < a.src_rows ? a.A + from * a.lda + 16 * chunk : p[2 + q];
+    }
+  }
+
+  // stage s of this tile (of the next one, counted on, from nk on), load q
+  __device__ __forceinline__ void issue(int s, int at_slot, int q) {
+    const bool over = s >= nk;
+    const int k = TK * (over ? s - nk : s) + 16 * chunk;
+    const int off = min(k, a.K - 16) - 16 * chunk;
+    load_lds16((over ? next[q] : src[q]) + off,
+               lds0 + (unsigned)(at_slot * STAGE + (q >> 1) * TM * TK + wave * 2048 + (q & 1) * 1024));
+  }
+
+  __device__ __forceinline__ void first_fragments() {
+    const int8_t* stg = sh.stage[slot];
+    const int at0 = 16 * (lk ^ ((lr >> 2) & 3));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) fa0[i] = *reinterpret_cast<const intx4*>(stg + (wm * 128 + i * 32 + lr) * TK + at0);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) fb0[j] = *reinterpret_cast<const intx4*>(stg + TM * TK + (wn * 64 + j * 32 + lr) * TK + at0);
+  }
+
+  // all stages of a tile; `after` is the next tile
+  template <int NB>
+  __device__ __forceinline__ void loop(const Job& after, int after_buf) {
+    constexpr int NJ = NB ? 2 : 0;  // a wavefront without rows only loads
+    const int pos = lk ^ ((lr >> 2) & 3);
+    const int a_off = (wm * 128 + lr) * TK, b_off = TM * TK + (wn * 64 + lr) * TK;
+    const int at0 = 16 * pos, at1 = 16 * (pos ^ 2);  // chunks lk and 2 + lk
+    intx4 fa1[4], fb1[2];
+    constexpr int MF = NB ? 2 * NB : 1, ACTS = NB + NJ + 2;  // matrix instructions of half a stage; reads and loads among them
+#pragma unroll 1
+    for (int kt = 0; kt < nk; ++kt) {
+      const int8_t* stg = sh.stage[slot];
+      const int before = (slot + NST - 1) % NST, here = slot;
+      slot = (slot + 1) % NST;
+      const int8_t* nxt = sh.stage[slot];
+      if (kt == 3) sources(after, after_buf, next);  // (the row numbers were loaded before kt = 0: landed by now)
+      const bool ragged = TK * (kt + 1) > a.K;
+      if (ragged) {
+        const int d = max(0, TK * kt + 16 * lk - (a.K - 16));
+#pragma unroll
+        for (int i = 0; i < NB; ++i) fa0[i] = keep_from(fa0[i], d);
+      }
+#pragma unroll
+      for (int m = 0; m < MF; ++m) {
+        if (NB) acc[m >> 1][m & 1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb0[m & 1], fa0[m >> 1], acc[m >> 1][m & 1], 0, 0, 0);
+#pragma unroll
+        for (int c = 0; c < ACTS; ++c)
+          if (c * MF / ACTS == m) {
+            if (c < NB) fa1[c] = *reinterpret_cast<const intx4*>(stg + a_off + at1 + c * 32 * TK);
+            else if (c < NB + NJ) fb1[c - NB] = *reinterpret_cast<const intx4*>(stg + b_off + at1 + (c - NB) * 32 * TK);
+            else issue(kt + NST - 1, before, 2 + c - NB - NJ);
+          }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(0x0070 | 8);  // the next stage landed: at most the 8 loads of the two after it in flight
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (ragged) {
+        const int d = max(0, TK * kt + 32 + 16 * lk - (a.K - 16));
+#pragma unroll
+        for (int i = 0; i < NB; ++i) fa1[i] = keep_from(fa1[i], d);
+      }
+#pragma unroll
+      for (int m = 0; m < MF; ++m) {
+        if (NB) acc[m >> 1][m & 1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb1[m & 1], fa1[m >> 1], acc[m >> 1][m & 1], 0, 0, 0);
+#pragma unroll
+        for (int c = 0; c < ACTS; ++c)
+          if (c * MF / ACTS == m) {
+            if (c < NB) fa0[c] = *reinterpret_cast<const intx4*>(nxt + a_off + at0 + c * 32 * TK);
+            else if (c < NB + NJ) fb0[c - NB] = *reinterpret_cast<const intx4*>(nxt + b_off + at0 + (c - NB) * 32 * TK);
+            else issue(kt + NST, here, c - NB - NJ);
+          }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void results(const Job& j, int buf) const {
+    const float* sb = a.sb + (long)j.e * (SWIGLU ? 2 * a.N : a.N);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = wm * 128 + i * 32 + lr, m = j.m0 + r;
+      if (m >= j.mend) continue;
+      const long from = a.rows ? sh.rows[buf][r] : m;
+      const float sa = from >= 0 && from < a.src_rows ? a.sa[from] : 0.f;
+#pragma unroll
+      for (int c0 = 0; c0 < (SWIGLU ? 1 : 2); ++c0)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int n = j.n0 + (SWIGLU ? wn * 32 : wn * 64 + c0 * 32) + 8 * g + 4 * lk;
+          float y[4];
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const int c = min(n + v, a.N - 1);
+            if (SWIGLU) {
+              y[v] = silu_times((float)acc[i][0][4 * g + v] * sa * sb[c], (float)acc[i][1][4 * g + v] * sa * sb[a.N + c]);
+            } else {
+              y[v] = (float)acc[i][c0][4 * g + v] * sa * sb[c];
+              if (a.bias) y[v] += load_val<DT>(a.bias, c);
+            }
+          }
+          store_run<DT>(a.Y, (long)m * a.ldy, n, a.N, a.vec_out, y);
+        }
+    }
+  }
+
+  // Jobs go to the XCDs (workgroup index mod 8) in turns, as many consecutive ones as an XCD has workgroups.  Whole tiles
+  // are bound by the matrix pipes, partly filled ones by the weights' bytes: every XCD gets an equal share of both and
+  // mixes them evenly, half of its workgroups half a turn later.
+  struct Order {
+    int per, jobs_w, jobs_p, at_w, at_p, turns, share, gone;
+    __device__ __forceinline__ Order(int2 tiles, int nt) {
+      const int xcd = blockIdx.x & 7, c = blockIdx.x >> 3;
+      per = gridDim.x >> 3;
+      jobs_w = tiles.x * nt;
+      jobs_p = tiles.y * nt;
+      const int tw = (jobs_w + per - 1) / per, tp = (jobs_p + per - 1) / per, xp = 7 - xcd;
+      share = tw > xcd ? (tw - xcd + 7) >> 3 : 0;                    // turns of this XCD with whole tiles
+      turns = share + (tp > xp ? (tp - xp + 7) >> 3 : 0);
+      at_w = xcd * per + c;
+      at_p = xp * per + c;
+      gone = c >= per / 2 ? turns >> 1 : 0;
+      left = turns;
+    }
+    int left;
+    __device__ __forceinline__ bool next(bool& whole, int& id) {
+      while (left > 0) {
+        --left;
+        gone += share;
+        whole = gone >= turns;
+        if (whole) gone -= turns;
+        id = whole ? at_w : at_p;
+        if (whole) at_w += 8 * per;
+        else at_p += 8 * per;
+        if (id < (whole ? jobs_w : jobs_p)) return true;
+      }
+      return false;
+    }
+  };
+
+  __device__ __forceinline__ void run() {
+    Order order(table(), (a.N + OUTN - 1) / OUTN);
+    bool whole;
+    int id;
+    if (!order.next(whole, id)) return;
+    Job now = job(whole, id);
+    int buf = 0;
+    if (a.rows) {
+      if (threadIdx.x < TM) sh.rows[0][threadIdx.x] = a.rows[min(now.m0 + (int)threadIdx.x, now.mend - 1)];
+      __syncthreads();
+    }
+    sources(now, 0, src);
+#pragma unroll
+    for (int s = 0; s < NST; ++s)
+#pragma unroll
+      for (int q = 0; q < (s < NST - 1 ? 4 : 2); ++q) issue(s, s, q);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070 | 10);  // stage 0 landed: at most the 10 loads of stages 1, 2, 3 in flight
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    for (;;) {
+      const bool more = order.next(whole, id);
+      const Job after = more ? job(whole, id) : now;  // (after the last tile its first stages are loaded again, for nobody)
+      const int buf1 = buf == 2 ? 0 : buf + 1;
+      if (a.rows)  // rows 32 wave .. 32 wave + 31, two words each
+        load_lds4((const int*)(a.rows + min(after.m0 + 32 * wave + (lane >> 1), after.mend - 1)) + (lane & 1),
+                  rows0 + (unsigned)(buf1 * TM + 32 * wave) * 8u);
+      first_fragments();
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) acc[i][j][v] = 0;
+      // (wavefronts of one workgroup may run different versions: loads, waits and barriers are the same in all)
+      const int rows = now.mend - now.m0 - wm * 128;
+      if (rows > 96) loop<4>(after, buf1);
+      else if (rows > 64) loop<3>(after, buf1);
+      else if (rows > 32) loop<2>(after, buf1);
+      else if (rows > 0) loop<1>(after, buf1);
+      else loop<0>(after, buf1);
+      results(now, buf);
+      if (!more) break;
+      now = after;
+      buf = buf1;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) src[q] = next[q];
+    }
+    __builtin_amdgcn_s_waitcnt(0x0070);
+  }
+};
+
 template <int DT, bool SWIGLU>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void int8_tile_kernel(Int8Args a) {
   extern __shared__ __attribute__((aligned(1024))) int8_t smem[];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave >> 2, wn = wave & 3;
-  constexpr int OUTN = SWIGLU ? TN / 2 : TN;
-  const int nt = (a.N + OUTN - 1) / OUTN;
-  int e = 0, m0, mend, tn;
-  if (a.offsets) {
-    const int tile = blockIdx.x / nt;
-    tn = blockIdx.x % nt;
-    if (!find_tile(a, tile, TM, e, m0, mend)) return;
-  } else {
-    // tiles in bands of eight row tiles, every XCD (workgroup index mod 8) a run of its own: the 32 tiles it works on share
-    // few panels
-    const int mt = (a.M + TM - 1) / TM, total = mt * nt;
-    const int xcd = blockIdx.x & 7, per = total >> 3, more = total & 7;
-    const int id = xcd * per + min(xcd, more) + (blockIdx.x >> 3);
-    const int band = id / (8 * nt), in = id - band * 8 * nt, rows = min(8, mt - 8 * band);
-    m0 = (8 * band + in % rows) * TM;
-    tn = in / rows;
-    mend = min(m0 + TM, a.M);
-  }
-  m0 = __builtin_amdgcn_readfirstlane(m0);
-  mend = __builtin_amdgcn_readfirstlane(mend);
-  e = __builtin_amdgcn_readfirstlane(e);
-  const int n0 = __builtin_amdgcn_readfirstlane(tn) * OUTN;
-  const int8_t* B = a.B + (long)e * a.strideB;
-  const float* sb = a.sb + (long)e * (SWIGLU ? 2 * a.N : a.N);
-  const int nk = (a.K + TK - 1) / TK;
+  TileKernel<DT, SWIGLU>(a, *reinterpret_cast<TileShared*>(smem)).run();
+}
 
-  // loads of this wavefront: rows 32 wave + 16 q + lane / 4 of the tokens (q = 0, 1) and of the weights (q = 2, 3)
-  const int chunk = (lane & 3) ^ (lane >> 4);
-  const int8_t* src[4];
-#pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    const int r = 32 * wave + 16 * q + (lane >> 2);
-    // SwiGLU: rows 0..31 of every 64 are gate rows, 32..63 the up rows of the same columns
-    int col = SWIGLU ? n0 + (r >> 6) * 32 + (r & 31) : n0 + r;
-    if (col >= a.N) col = n0;
-    src[2 + q] = B + (long)(SWIGLU && (r & 32) ? a.N + col : col) * a.ldb + 16 * chunk;
-    long from = min(m0 + r, mend - 1);
-    if (a.rows) from = a.rows[from];
-    src[q] = from >= 0 && from < a.src_rows ? a.A + from * a.lda + 16 * chunk : src[2 + q];
+template <int DT, bool SWIGLU>
+int tile_launch(const Int8Args& a, hipStream_t st) {
+  static std::atomic<int> cus[64];  // per GPU: its CUs, once the kernel may take its shared memory there
+  int dev = -1;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return MQ_ERR_LAUNCH;
+  int n = cus[dev].load();
+  if (n == 0) {
+    if (hipFuncSetAttribute((const void*)int8_tile_kernel<DT, SWIGLU>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                            (int)sizeof(TileShared)) != hipSuccess ||
+        hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 8)
+      return MQ_ERR_LAUNCH;
+    n &= ~7;  // the same number on every XCD
+    cus[dev].store(n);
   }
-  const int last = TK * (nk - 1) + 16 * chunk;      // this lane's chunk of the last stage starts here
-  const int back = max(0, last - (a.K - 16));       // and is loaded from this much before
-  const unsigned lds0 = __builtin_amdgcn_readfirstlane(
-      (unsigned)(uintptr_t)(__attribute__((address_space(3))) int8_t*)smem);
-  // (stages past the last one load the last one's bytes again into slots nobody reads: the waits keep their counts)
-  auto issue = [&](int s, int q) {
-    const int off = s < nk - 1 ? TK * s : TK * (nk - 1) - back;
-    load_lds16(src[q] + off, lds0 + (unsigned)((s % NST) * STAGE + (q >> 1) * TM * TK + wave * 2048 + (q & 1) * 1024));
-  };
-
-  intx16 acc[4][2];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) acc[i][j][v] = 0;
-#pragma unroll
-  for (int s = 0; s < NST - 1; ++s)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) issue(s, q);
-#pragma unroll
-  for (int q = 0; q < 2; ++q) issue(NST - 1, q);
-
-  const int lr = lane & 31, lk = lane >> 5;
-  const int pos = lk ^ ((lr >> 2) & 3);
-  const int a_off = (wm * 128 + lr) * TK, b_off = TM * TK + (wn * 64 + lr) * TK;
-  const int at0 = 16 * pos, at1 = 16 * (pos ^ 2);  // chunks lk and 2 + lk
-  intx4 fa0[4], fb0[2], fa1[4], fb1[2];
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0x0070 | 10);  // stage 0 landed: at most the 10 loads of stages 1, 2, 3 in flight
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 4; ++i) fa0[i] = *reinterpret_cast<const intx4*>(smem + a_off + at0 + i * 32 * TK);
-#pragma unroll
-  for (int j = 0; j < 2; ++j) fb0[j] = *reinterpret_cast<const intx4*>(smem + b_off + at0 + j * 32 * TK);
-#pragma unroll 1
-  for (int kt = 0; kt < nk; ++kt) {
-    const int8_t* stg = smem + (kt % NST) * STAGE;
-    const int8_t* nxt = smem + ((kt + 1) % NST) * STAGE;
-    const bool ragged = kt == nk - 1 && (a.K % TK);
-    if (ragged) {
-      const int d = max(0, TK * (nk - 1) + 16 * lk - (a.K - 16));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) fa0[i] = keep_from(fa0[i], d);
-    }
-#pragma unroll
-    for (int m = 0; m < 8; ++m) {
-      acc[m >> 1][m & 1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb0[m & 1], fa0[m >> 1], acc[m >> 1][m & 1], 0, 0, 0);
-      if (m < 4) fa1[m] = *reinterpret_cast<const intx4*>(stg + a_off + at1 + m * 32 * TK);
-      else if (m < 6) fb1[m - 4] = *reinterpret_cast<const intx4*>(stg + b_off + at1 + (m - 4) * 32 * TK);
-      else issue(kt + NST - 1, 2 + (m - 6));
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0070 | 8);  // stage kt+1 landed: at most the 8 loads of stages kt+2, kt+3 in flight
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (ragged) {
-      const int d = max(0, TK * (nk - 1) + 32 + 16 * lk - (a.K - 16));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) fa1[i] = keep_from(fa1[i], d);
-    }
-#pragma unroll
-    for (int m = 0; m < 8; ++m) {
-      acc[m >> 1][m & 1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb1[m & 1], fa1[m >> 1], acc[m >> 1][m & 1], 0, 0, 0);
-      if (m < 4) fa0[m] = *reinterpret_cast<const intx4*>(nxt + a_off + at0 + m * 32 * TK);
-      else if (m < 6) fb0[m - 4] = *reinterpret_cast<const intx4*>(nxt + b_off + at0 + (m - 4) * 32 * TK);
-      else issue(kt + NST, m - 6);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  }
-  __builtin_amdgcn_s_waitcnt(0x0070);
-
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int m = m0 + wm * 128 + i * 32 + lr;
-    if (m >= mend) continue;
-    long from = m;
-    if (a.rows) from = a.rows[m];
-    const float sa = from >= 0 && from < a.src_rows ? a.sa[from] : 0.f;
-#pragma unroll
-    for (int j = 0; j < (SWIGLU ? 1 : 2); ++j)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int n = n0 + (SWIGLU ? wn * 32 : wn * 64 + j * 32) + 8 * g + 4 * lk;
-        float y[4];
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const int c = min(n + v, a.N - 1);
-          if (SWIGLU) {
-            y[v] = silu_times((float)acc[i][0][4 * g + v] * sa * sb[c], (float)acc[i][1][4 * g + v] * sa * sb[a.N + c]);
-          } else {
-            y[v] = (float)acc[i][j][4 * g + v] * sa * sb[c];
-            if (a.bias) y[v] += load_val<DT>(a.bias, c);
-          }
-        }
-        store_run<DT>(a.Y, (long)m * a.ldy, n, a.N, a.vec_out, y);
-      }
-  }
+  const long mt = a.offsets ? (long)a.M / TM + min(a.E, a.M) : ((long)a.M + TM - 1) / TM;
+  const int outn = SWIGLU ? TN / 2 : TN;
+  const long jobs = mt * ((a.N + outn - 1) / outn);
+  if (jobs > 0x7fffffffL) return MQ_ERR_TOO_LARGE;
+  const int grid = (int)min((long)n, (jobs + 7) / 8 * 8);
+  hipLaunchKernelGGL((int8_tile_kernel<DT, SWIGLU>), dim3(grid), dim3(512), sizeof(TileShared), st, a);
+  return mq_check_launch();
 }
 
 bool rows_of_words(const int8_t* p, long ld) { return ((uintptr_t)p & 3) == 0 && ld % 4 == 0; }
@@ -445,19 +763,7 @@ bool rows_of_words(const int8_t* p, long ld) { return ((uintptr_t)p & 3) == 0 &&
 template <int DT, bool SWIGLU>
 int int8_launch(const Int8Args& a, hipStream_t st) {
   if (a.K >= 16 && a.M >= 64 && rows_of_words(a.A, a.lda) && rows_of_words(a.B, a.ldb) && a.strideB % 4 == 0) {
-    static std::once_flag once;
-    static bool ok = false;
-    std::call_once(once, [] {
-      ok = hipFuncSetAttribute((const void*)int8_tile_kernel<DT, SWIGLU>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)TILE_SMEM) == hipSuccess;
-    });
-    if (!ok) return MQ_ERR_LAUNCH;
-    const long mt = a.offsets ? (long)a.M / TM + min(a.E, a.M) : ((long)a.M + TM - 1) / TM;
-    const int outn = SWIGLU ? TN / 2 : TN;
-    const long grid = mt * ((a.N + outn - 1) / outn);
-    if (grid > 0x7fffffffL) return MQ_ERR_TOO_LARGE;
-    hipLaunchKernelGGL((int8_tile_kernel<DT, SWIGLU>), dim3((unsigned)grid), dim3(512), TILE_SMEM, st, a);
-    return mq_check_launch();
+    return tile_launch<DT, SWIGLU>(a, st);
   }
   const long mt = a.offsets ? (long)a.M / GBM + min(a.E, a.M) : ((long)a.M + GBM - 1) / GBM;
   const int outn = SWIGLU ? GBN / 2 : GBN;
@@ -486,12 +792,9 @@ extern "C" int mq_quantize_tokens(const void* X, int dtype, long ldx, int n, int
   if (n == 0) return MQ_OK;
   if (!X || !Q || !scale) return MQ_ERR_ARG;
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == DT_F32)
-    hipLaunchKernelGGL((quantize_tokens_kernel<DT_F32>), dim3(n), dim3(256), 0, st, X, ldx, C, Q, ldq, scale);
-  else if (dtype == DT_BF16)
-    hipLaunchKernelGGL((quantize_tokens_kernel<DT_BF16>), dim3(n), dim3(256), 0, st, X, ldx, C, Q, ldq, scale);
-  else
-    hipLaunchKernelGGL((quantize_tokens_kernel<DT_F16>), dim3(n), dim3(256), 0, st, X, ldx, C, Q, ldq, scale);
+  if (dtype == DT_F32) quantize_launch<DT_F32>(X, ldx, n, C, Q, ldq, scale, st);
+  else if (dtype == DT_BF16) quantize_launch<DT_BF16>(X, ldx, n, C, Q, ldq, scale, st);
+  else quantize_launch<DT_F16>(X, ldx, n, C, Q, ldq, scale, st);
   return mq_check_launch();
 }
 
