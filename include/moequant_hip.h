@@ -349,13 +349,20 @@ int mq_quantize_tokens(const void* X, int dtype, long ldx, int n, int C, int8_t*
 /* Y[m, n] = (sum_k A[m, k] * B[n, k]) * a_scale[m] * b_scale[n] + bias[n]: the sum in 32-bit integers (exact), the rest in
  * fp32, rounded once to out_dtype.  A : M x K (lda), B : N x K (ldb), Y : M x N (ldy), bias (nullable) : N values of
  * out_dtype.  swiglu != 0: B holds 2 N rows (N gate rows, then N up rows; b_scale 2 N values, no bias) and
- * Y[m, n] = silu(gate) * up, rounded once.  K <= 131071.  Any alignment; 16-byte aligned rows (pointers and pitches of
- * A and B multiples of 16) run fastest.
+ * Y[m, n] = silu(gate) * up, rounded once.  K <= 131071.  Any alignment; rows that start at multiples of 4
+ * (pointers and pitches of A and B) run fastest.
  *   workspace: mq_matmul_int8_workspace_bytes(M, N, K, swiglu) bytes, 16-byte aligned (0: none needed). */
 size_t mq_matmul_int8_workspace_bytes(int M, int N, int K, int swiglu);
 int mq_matmul_int8(const int8_t* A, long lda, const float* a_scale, const int8_t* B, long ldb, const float* b_scale,
                    const void* bias, void* Y, long ldy, int out_dtype, int M, int N, int K, int swiglu, void* workspace,
                    size_t workspace_bytes, void* stream);
+
+/* mq_quantize_tokens and mq_matmul_int8 in one call: Y = the linear layer (B, b_scale, bias) on X : M x K (ldx), Y and
+ * bias of X's type.  One launch for one or two tokens.
+ *   workspace: mq_linear_int8_workspace_bytes(M, N, K) bytes, 16-byte aligned (0: none needed). */
+size_t mq_linear_int8_workspace_bytes(int M, int N, int K);
+int mq_linear_int8(const void* X, int dtype, long ldx, const int8_t* B, long ldb, const float* b_scale, const void* bias,
+                   void* Y, long ldy, int M, int N, int K, void* workspace, size_t workspace_bytes, void* stream);
 
 /* The same with weights per run of rows: rows offsets[e] .. offsets[e + 1) - 1 of Y (device array of E + 1 values, clamped
  * to [0, S]) are products with B + e * strideB, b_scale + e * N (swiglu: e * 2 N).  Row m of Y takes row rows[m] of A and

@@ -60,6 +60,8 @@ SIGNATURES = {
     "mq_quantize_tokens": (_i, [_vp, _i, _l, _i, _i, _vp, _l, _vp, _vp]),
     "mq_matmul_int8_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "mq_matmul_int8": (_i, [_vp, _l, _vp, _vp, _l, _vp, _vp, _vp, _l, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "mq_linear_int8_workspace_bytes": (_sz, [_i, _i, _i]),
+    "mq_linear_int8": (_i, [_vp, _i, _l, _vp, _l, _vp, _vp, _vp, _l, _i, _i, _i, _vp, _sz, _vp]),
     "mq_matmul_int8_grouped": (_i, [_vp, _l, _vp, _i, _vp, _i, _vp, _l, _l, _vp, _i, _vp, _vp, _l, _i, _i, _i, _i, _vp]),
     "mq_gemm_f32": (_i, [_vp, _l, _l, _vp, _l, _l, _vp, _l, _i, _i, _i, _f, _f, _i, _i, _vp]),
 }

@@ -190,60 +190,6 @@ struct Int8Args {
   int vec_out;
 };
 
-// Row tiles of a grouped product: the experts' tiles of bm rows follow one another.  `locate` finds the workgroup's own:
-// a lane counts the tiles of E / 64 consecutive experts, a prefix sum over the lanes gives the number of tiles in all and
-// the lane that holds the wanted one.  Offsets are clamped to [0, M].
-struct RowTiles {
-  int first, per;  // this lane's experts
-  int before, total;
-
-  __device__ __forceinline__ static void range(const Int8Args& a, int e, int& lo, int& hi) {
-    lo = (int)min(max(a.offsets[e], 0l), (long)a.M);
-    hi = (int)min(max(a.offsets[e + 1], (long)lo), (long)a.M);
-  }
-  __device__ __forceinline__ void count(const Int8Args& a, int bm) {
-    const int lane = threadIdx.x & 63;
-    per = (a.E + 63) >> 6;
-    first = lane * per;
-    int mine = 0;
-    for (int i = 0; i < per; ++i) {
-      const int e = first + i;
-      if (e < a.E) {
-        int lo, hi;
-        range(a, e, lo, hi);
-        mine += (hi - lo + bm - 1) / bm;
-      }
-    }
-    int s = mine;
-    for (int o = 1; o < 64; o <<= 1) {
-      const int u = __shfl_up(s, o);
-      if (lane >= o) s += u;
-    }
-    before = s - mine;
-    total = __builtin_amdgcn_readlane(s, 63);
-  }
-  // tile < total: its expert and rows m0 .. mend - 1
-  __device__ __forceinline__ void locate(const Int8Args& a, int bm, int tile, int& e_out, int& m0, int& mend) const {
-    const int lane = threadIdx.x & 63;
-    const unsigned long who = __ballot(before <= tile);  // lanes 0 .. the one that holds it
-    const int src = 63 - __builtin_clzll(who);
-    int left = tile - __builtin_amdgcn_readlane(before, src);
-    int e = src * per;
-    for (;; ++e) {
-      int lo, hi;
-      range(a, e, lo, hi);
-      const int tiles = (hi - lo + bm - 1) / bm;
-      if (left < tiles || e + 1 >= a.E) {
-        e_out = e;
-        m0 = lo + left * bm;
-        mend = min(m0 + bm, hi);
-        return;
-      }
-      left -= tiles;
-    }
-  }
-};
-
 // four results of one row, columns n .. n + 3, as far as they exist
 template <int DT>
 __device__ __forceinline__ void store_run(void* Y, long row, int n, int N, int vec, const float* y) {
@@ -268,123 +214,14 @@ __device__ __forceinline__ void store_run(void* Y, long row, int n, int N, int v
 
 __device__ __forceinline__ float silu_times(float g, float u) { return g / (1.f + __expf(-g)) * u; }
 
-// 16 bytes of a row from byte k on, zeros beyond K (any alignment)
-__device__ __forceinline__ intx4 load16(const int8_t* row, int k, int K, bool in) {
-  intx4 v = {0, 0, 0, 0};
-  if (!in || k >= K) return v;
-  if (k + 16 <= K) {
-    __builtin_memcpy(&v, row + k, 16);
-  } else {
-    int8_t* b = reinterpret_cast<int8_t*>(&v);
-    for (int i = 0; i < 16; ++i) b[i] = k + i < K ? row[k + i] : (int8_t)0;
-  }
+// bytes k .. k + 15 of a row of fewer than 16, zeros beyond its end
+__device__ __forceinline__ intx4 short_row(const int8_t* row, int k, int K, bool in) {
+  int8_t b[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) b[i] = in && k + i < K ? row[k + i] : (int8_t)0;
+  intx4 v;
+  __builtin_memcpy(&v, b, 16);
   return v;
-}
-
-// Any sizes, strides and alignment: 128 x 128 tiles, 64 deep, staged through registers and shared memory; four wavefronts
-// of 64 x 64.  The weights are the matrix instruction's first operand, so a lane holds runs of four columns of one row.
-constexpr int GBM = 128, GBN = 128, GBK = 64, GLD = GBK + 16;
-template <int DT, bool SWIGLU>
-__global__ __launch_bounds__(256) void int8_any_kernel(Int8Args a) {
-  __shared__ __attribute__((aligned(16))) int8_t As[GBM * GLD];
-  __shared__ __attribute__((aligned(16))) int8_t Bs[GBN * GLD];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int wm = wave >> 1, wn = wave & 1;
-  int e = 0, m0 = blockIdx.y * GBM, mend = min(m0 + GBM, a.M);
-  if (a.offsets) {
-    RowTiles t;
-    t.count(a, GBM);
-    if ((int)blockIdx.y >= t.total) return;
-    t.locate(a, GBM, blockIdx.y, e, m0, mend);
-  }
-  constexpr int OUTN = SWIGLU ? GBN / 2 : GBN;
-  const int n0 = blockIdx.x * OUTN;
-  const int8_t* B = a.B + (long)e * a.strideB;
-  const float* sb = a.sb + (long)e * (SWIGLU ? 2 * a.N : a.N);
-
-  // this thread stages rows tid / 4 and tid / 4 + 64 of both tiles, 16 bytes at 16 * (tid % 4)
-  const int8_t *arow[2], *brow[2];
-  bool ain[2], bin[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int r = (tid >> 2) + 64 * h;
-    long src = m0 + r;
-    ain[h] = m0 + r < mend;
-    if (ain[h] && a.rows) {
-      src = a.rows[src];
-      ain[h] = src >= 0 && src < a.src_rows;
-    }
-    arow[h] = a.A + (ain[h] ? src : 0) * a.lda;
-    // SwiGLU: rows 0..31 of every 64 are gate rows, 32..63 the up rows of the same columns
-    const int col = SWIGLU ? n0 + (r >> 6) * 32 + (r & 31) : n0 + r;
-    bin[h] = col < a.N;
-    brow[h] = B + (long)(bin[h] ? (SWIGLU && (r & 32) ? a.N + col : col) : 0) * a.ldb;
-  }
-  intx16 acc[2][2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) acc[i][j][v] = 0;
-  const int kc = 16 * (tid & 3);
-  for (int k0 = 0; k0 < a.K; k0 += GBK) {
-    intx4 va[2], vb[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      va[h] = load16(arow[h], k0 + kc, a.K, ain[h]);
-      vb[h] = load16(brow[h], k0 + kc, a.K, bin[h]);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = (tid >> 2) + 64 * h;
-      *reinterpret_cast<intx4*>(As + r * GLD + kc) = va[h];
-      *reinterpret_cast<intx4*>(Bs + r * GLD + kc) = vb[h];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int kk = 0; kk < GBK; kk += 32) {
-      intx4 fa[2], fb[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        fa[i] = *reinterpret_cast<const intx4*>(As + (wm * 64 + i * 32 + (lane & 31)) * GLD + kk + 16 * (lane >> 5));
-        fb[i] = *reinterpret_cast<const intx4*>(Bs + (wn * 64 + i * 32 + (lane & 31)) * GLD + kk + 16 * (lane >> 5));
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[j], fa[i], acc[i][j], 0, 0, 0);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int m = m0 + wm * 64 + i * 32 + (lane & 31);
-    if (m >= mend) continue;
-    long src = m;
-    if (a.rows) src = a.rows[m];
-    const float sa = src >= 0 && src < a.src_rows ? a.sa[src] : 0.f;
-    if (SWIGLU) {
-#pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        const int n = n0 + wn * 32 + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3);
-        if (n >= a.N) continue;
-        const float g = (float)acc[i][0][v] * sa * sb[n], u = (float)acc[i][1][v] * sa * sb[a.N + n];
-        store_val<DT>(a.Y, (long)m * a.ldy + n, silu_times(g, u));
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const int n = n0 + wn * 64 + j * 32 + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3);
-          if (n >= a.N) continue;
-          float y = (float)acc[i][j][v] * sa * sb[n];
-          if (a.bias) y += load_val<DT>(a.bias, n);
-          store_val<DT>(a.Y, (long)m * a.ldy + n, y);
-        }
-    }
-  }
 }
 
 // Tiles of 256 x 256 for rows of at least 16 bytes that start at multiples of 4.  One workgroup per CU, eight wavefronts of
@@ -758,27 +595,421 @@ int tile_launch(const Int8Args& a, hipStream_t st) {
   return mq_check_launch();
 }
 
-bool rows_of_words(const int8_t* p, long ld) { return ((uintptr_t)p & 3) == 0 && ld % 4 == 0; }
-
-template <int DT, bool SWIGLU>
-int int8_launch(const Int8Args& a, hipStream_t st) {
-  if (a.K >= 16 && a.M >= 64 && rows_of_words(a.A, a.lda) && rows_of_words(a.B, a.ldb) && a.strideB % 4 == 0) {
-    return tile_launch<DT, SWIGLU>(a, st);
+// Few rows or few tiles: a workgroup computes 16 R x 16 C results, its eight wavefronts an eighth of K each, with fragments
+// straight from memory (16 rows x 64 bytes an instruction, UN of them in flight) -- every weight byte of the tile is used by
+// one wavefront only, so shared memory would add nothing but latency.  The eight sums meet in shared memory.  Grouped: a
+// workgroup belongs to an expert and walks over its rows in steps of 16 R.  Any alignment, any K.
+template <int DT, bool SWIGLU, int R, int C, int UN>
+__global__ __launch_bounds__(512) void int8_thin_kernel(Int8Args a, int gx) {
+  __shared__ intx4 part[8][R * C][64];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l16 = lane & 15, lq = lane >> 4;
+  constexpr int OUTN = SWIGLU ? 8 * C : 16 * C;
+  const int by = blockIdx.x / gx, n0 = (blockIdx.x - by * gx) * OUTN;
+  int e = 0, mbeg = by * 16 * R, mend = min(mbeg + 16 * R, a.M);
+  if (a.offsets) {
+    e = by;
+    mbeg = (int)min(max(a.offsets[e], 0l), (long)a.M);
+    mend = (int)min(max(a.offsets[e + 1], (long)mbeg), (long)a.M);
   }
-  const long mt = a.offsets ? (long)a.M / GBM + min(a.E, a.M) : ((long)a.M + GBM - 1) / GBM;
-  const int outn = SWIGLU ? GBN / 2 : GBN;
-  if (mt > 65535) return MQ_ERR_TOO_LARGE;
-  hipLaunchKernelGGL((int8_any_kernel<DT, SWIGLU>), dim3((a.N + outn - 1) / outn, (unsigned)mt), dim3(256), 0, st, a);
+  const int8_t* B = a.B + (long)e * a.strideB;
+  const float* sb = a.sb + (long)e * (SWIGLU ? 2 * a.N : a.N);
+  const int steps = (a.K + 63) >> 6, per = (steps + 7) >> 3;
+  const int k0 = 64 * per * wave, k1 = min(a.K, k0 + 64 * per);
+  const int8_t* brow[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    // SwiGLU: even blocks of 16 are gate rows, odd ones the up rows of the same columns
+    int col = SWIGLU ? n0 + 16 * (c >> 1) + l16 : n0 + 16 * c + l16;
+    if (col >= a.N) col = n0;
+    brow[c] = B + (long)(SWIGLU && (c & 1) ? a.N + col : col) * a.ldb;
+  }
+  for (int m0 = mbeg; m0 < mend; m0 += 16 * R) {
+    const int8_t* arow[R];
+    bool ain[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int m = m0 + 16 * r + l16;
+      long from = m;
+      ain[r] = m < mend;
+      if (ain[r] && a.rows) from = a.rows[m];
+      ain[r] = ain[r] && from >= 0 && from < a.src_rows;
+      arow[r] = a.A + (ain[r] ? from : 0) * a.lda;
+    }
+    intx4 acc[R][C];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int c = 0; c < C; ++c) acc[r][c] = intx4{0, 0, 0, 0};
+    for (int k = k0; k < k1; k += 64 * UN) {
+      intx4 fa[UN][R], fb[UN][C];
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        // chunks beyond the end of a row: the weights' last 16 bytes once more, against zeros
+        const int kc = k + 64 * u + 16 * lq, at = min(kc, a.K - 16);
+        if (a.K < 16) {
+#pragma unroll
+          for (int c = 0; c < C; ++c) fb[u][c] = short_row(brow[c], kc, a.K, true);
+#pragma unroll
+          for (int r = 0; r < R; ++r) fa[u][r] = short_row(arow[r], kc, a.K, ain[r]);
+          continue;
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c) __builtin_memcpy(&fb[u][c], brow[c] + at, 16);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          fa[u][r] = intx4{0, 0, 0, 0};
+          if (ain[r] && kc < k1) __builtin_memcpy(&fa[u][r], arow[r] + at, 16);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        const int kc = k + 64 * u + 16 * lq;
+        if ((a.K & 15) && a.K > 16) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) fa[u][r] = keep_from(fa[u][r], kc - (a.K - 16));
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+            acc[r][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[u][c], fa[u][r], acc[r][c], 0, 0, 0);
+      }
+    }
+    if (m0 != mbeg) __syncthreads();  // the sums of the rows before have been read
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int c = 0; c < C; ++c) part[wave][r * C + c][lane] = acc[r][c];
+    __syncthreads();
+    constexpr int CB = SWIGLU ? C / 2 : C, ITEMS = R * CB * 64;
+    for (int it = tid; it < ITEMS; it += 512) {
+      const int ln = it & 63, r = (it >> 6) / CB, c = (it >> 6) % CB;
+      const int m = m0 + 16 * r + (ln & 15), n = n0 + 16 * c + 4 * (ln >> 4);
+      if (m >= mend || n >= a.N) continue;
+      long from = m;
+      if (a.rows) from = a.rows[m];
+      const float sa = from >= 0 && from < a.src_rows ? a.sa[from] : 0.f;
+      intx4 s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        s0 += part[w][r * C + (SWIGLU ? 2 * c : c)][ln];
+        if (SWIGLU) s1 += part[w][r * C + 2 * c + 1][ln];
+      }
+      float y[4];
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int col = min(n + v, a.N - 1);
+        if (SWIGLU) {
+          y[v] = silu_times((float)s0[v] * sa * sb[col], (float)s1[v] * sa * sb[a.N + col]);
+        } else {
+          y[v] = (float)s0[v] * sa * sb[col];
+          if (a.bias) y[v] += load_val<DT>(a.bias, col);
+        }
+      }
+      store_run<DT>(a.Y, (long)m * a.ldy, n, a.N, a.vec_out, y);
+    }
+  }
+}
+
+template <int DT, bool SWIGLU, int R, int C, int UN>
+int thin_launch(const Int8Args& a, hipStream_t st) {
+  const int outn = SWIGLU ? 8 * C : 16 * C, gx = (a.N + outn - 1) / outn;
+  const long grid = (long)gx * (a.offsets ? a.E : (a.M + 16 * R - 1) / (16 * R));
+  if (grid > 0x7fffffffL) return MQ_ERR_TOO_LARGE;
+  hipLaunchKernelGGL((int8_thin_kernel<DT, SWIGLU, R, C, UN>), dim3((unsigned)grid), dim3(512), 0, st, a, gx);
   return mq_check_launch();
 }
 
-int int8_dispatch(Int8Args a, int dtype, int swiglu, hipStream_t st) {
+// One or two rows: the weights' bytes are all that counts.  A wavefront streams pairs of weight rows (SwiGLU: a gate row and
+// its up row), 1 KB of a row an instruction, up to sixteen of them in flight; the tokens' codes lie in shared memory and
+// meet the weights in four-byte dot products.  Tokens come as codes (XDT < 0) or are quantized here by every workgroup for
+// itself (XDT = their type), under the first weights' way from memory.  Any alignment; K of at least 16.
+//   A row's last chunk, where K is no multiple of 16, is its last 16 bytes, and the tokens' bytes that belong to the chunk
+//   before are zero there.
+constexpr int VT = 2, VEC_THREADS = 256, VEC_CHUNKS = 8;
+
+template <int DT, bool SWIGLU, int XDT>
+struct VectorKernel {
+  const Int8Args& a;
+  int8_t* codes;  // VT rows of 16 ceil(K / 16) bytes
+  float* scales;  // VT
+  float* red;     // a value a wavefront
+  const int lane, wave, chunks, pitch;
+
+  __device__ __forceinline__ VectorKernel(const Int8Args& args, int8_t* smem)
+      : a(args), codes(smem), lane(threadIdx.x & 63), wave(threadIdx.x >> 6), chunks((args.K + 15) >> 4), pitch(chunks * 16) {}
+
+  __device__ __forceinline__ const int8_t* weight_row(int n, int second) const {
+    const int r = SWIGLU ? (second ? a.N + n : n) : min(n + second, a.N - 1);
+    return a.B + (long)r * a.ldb;
+  }
+  __device__ __forceinline__ void load(const int8_t* w0, const int8_t* w1, int c0, intx4 (*v)[2]) const {
+#pragma unroll
+    for (int u = 0; u < VEC_CHUNKS; ++u) {
+      const int at = min(16 * min(c0 + 64 * u + lane, chunks - 1), a.K - 16);
+      if (64 * (c0 / 64 + u) < chunks) {
+        __builtin_memcpy(&v[u][0], w0 + at, 16);
+        __builtin_memcpy(&v[u][1], w1 + at, 16);
+      }
+    }
+  }
+
+  // the tokens' codes and scales into shared memory
+  __device__ __forceinline__ void stage() {
+    for (int r = 0; r < a.M; ++r) {
+      int8_t* q = codes + r * pitch;
+      if (XDT < 0) {
+        const int8_t* p = a.A + (long)r * a.lda;
+        for (int c = threadIdx.x; c < chunks; c += VEC_THREADS) {
+          intx4 v;
+          __builtin_memcpy(&v, p + min(16 * c, a.K - 16), 16);
+          *reinterpret_cast<intx4*>(q + 16 * c) = keep_from(v, 16 * c - (a.K - 16));
+        }
+        if (threadIdx.x == 0) scales[r] = a.sa[r];
+      } else {
+        constexpr int D = XDT < 0 ? 0 : XDT;
+        const void* x0 = (const char*)a.A + (long)r * a.lda * (D == DT_F32 ? 4 : 2);
+        constexpr int KEEP = 4;  // vectors of eight kept in registers; longer rows are read twice
+        float x[KEEP][8];
+        float top = 0.f;
+        auto look = [&](const float* v) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) top = v[i] == v[i] ? fmaxf(top, fabsf(v[i])) : INFINITY;
+        };
+#pragma unroll
+        for (int v = 0; v < KEEP; ++v) load8<D>(x0, (v * VEC_THREADS + threadIdx.x) * 8, a.K, x[v]);
+#pragma unroll
+        for (int v = 0; v < KEEP; ++v) look(x[v]);
+        for (int c = (KEEP * VEC_THREADS + threadIdx.x) * 8; c < a.K; c += 8 * VEC_THREADS) {
+          float y[8];
+          load8<D>(x0, c, a.K, y);
+          look(y);
+        }
+        for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+        if (r) __syncthreads();
+        if (lane == 0) red[wave] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        const bool fine = top <= 3.402823466e38f, zero = !fine || top == 0.f;
+        if (threadIdx.x == 0) scales[r] = fine ? top / 127.f : NAN;
+        const float up = top < 0x1p-90f ? 0x1p90f : 1.f;
+        top *= up;
+        const float inv = zero ? 0.f : 127.f / top;
+        auto put = [&](float* v, int c) {
+          if (c >= a.K) return;
+          if (zero || up != 1.f) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = zero ? 0.f : v[i] * up;
+          }
+          const uint2 w = eight_codes(v, top, inv);
+          const int whole = a.K & ~15;
+          if (c + 8 <= whole) {
+            *reinterpret_cast<uint2*>(q + c) = w;
+          } else {  // the last chunk starts at K - 16
+            int8_t b[8];
+            __builtin_memcpy(b, &w, 8);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (c + i < a.K) q[whole + c + i - (a.K - 16)] = b[i];
+          }
+        };
+        if ((a.K & 15) && threadIdx.x < 16 - (a.K & 15)) q[(a.K & ~15) + threadIdx.x] = 0;
+#pragma unroll
+        for (int v = 0; v < KEEP; ++v) put(x[v], (v * VEC_THREADS + threadIdx.x) * 8);
+        for (int c = (KEEP * VEC_THREADS + threadIdx.x) * 8; c < a.K; c += 8 * VEC_THREADS) {
+          float y[8];
+          load8<D>(x0, c, a.K, y);
+          put(y, c);
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void finish(int m, int n, int second, int sum0, int sum1) const {
+    const float sa = scales[m];
+    if (SWIGLU) {
+      store_val<DT>(a.Y, (long)m * a.ldy + n, silu_times((float)sum0 * sa * a.sb[n], (float)sum1 * sa * a.sb[a.N + n]));
+    } else if (n + second < a.N) {
+      float y = (float)(second ? sum1 : sum0) * sa * a.sb[n + second];
+      if (a.bias) y += load_val<DT>(a.bias, n + second);
+      store_val<DT>(a.Y, (long)m * a.ldy + n + second, y);
+    }
+  }
+
+  template <int MT>
+  __device__ __forceinline__ void dots(const intx4 (*v)[2], int c0, int (*acc)[2]) const {
+#pragma unroll
+    for (int u = 0; u < VEC_CHUNKS; ++u) {
+      const int c = c0 + 64 * u + lane;
+      if (c < chunks) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const intx4 q = *reinterpret_cast<const intx4*>(codes + m * pitch + 16 * c);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            acc[m][0] = __builtin_amdgcn_sdot4(v[u][0][i], q[i], acc[m][0], false);
+            acc[m][1] = __builtin_amdgcn_sdot4(v[u][1][i], q[i], acc[m][1], false);
+          }
+        }
+      }
+    }
+  }
+
+  // one pair of weight rows against MT tokens; v holds the first chunks already
+  template <int MT>
+  __device__ __forceinline__ void pair(int n, intx4 (*v)[2]) const {
+    int acc[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[m][0] = acc[m][1] = 0;
+    const int8_t *w0 = weight_row(n, 0), *w1 = weight_row(n, 1);
+    dots<MT>(v, 0, acc);
+    for (int c0 = 64 * VEC_CHUNKS; c0 < chunks; c0 += 64 * VEC_CHUNKS) {
+      load(w0, w1, c0, v);
+      dots<MT>(v, c0, acc);
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      int s0 = acc[m][0], s1 = acc[m][1];
+      for (int o = 32; o; o >>= 1) {
+        s0 += __shfl_xor(s0, o);
+        s1 += __shfl_xor(s1, o);
+      }
+      if (lane < (SWIGLU ? 1 : 2)) finish(m, n, lane, s0, s1);
+    }
+  }
+
+  __device__ __forceinline__ void run() {
+    scales = reinterpret_cast<float*>(codes + VT * pitch);
+    red = scales + VT;
+    constexpr int WIDTH = SWIGLU ? 1 : 2;
+    const int pairs = (a.N + WIDTH - 1) / WIDTH;
+    const int first = blockIdx.x * (VEC_THREADS / 64) + wave, step = gridDim.x * (VEC_THREADS / 64);
+    intx4 v[VEC_CHUNKS][2];
+    if (first < pairs) load(weight_row(first * WIDTH, 0), weight_row(first * WIDTH, 1), 0, v);
+    stage();
+    __syncthreads();
+    for (int p = first; p < pairs; p += step) {
+      if (p != first) load(weight_row(p * WIDTH, 0), weight_row(p * WIDTH, 1), 0, v);
+      if (a.M > 1) pair<2>(p * WIDTH, v);
+      else pair<1>(p * WIDTH, v);
+    }
+  }
+};
+
+template <int DT, bool SWIGLU, int XDT>
+__global__ __launch_bounds__(VEC_THREADS) void int8_vector_kernel(Int8Args a) {
+  extern __shared__ __attribute__((aligned(1024))) int8_t smem[];
+  VectorKernel<DT, SWIGLU, XDT>(a, smem).run();
+}
+
+size_t vector_smem(int K) { return (size_t)VT * ((K + 15) / 16 * 16) + (VT + 8) * sizeof(float); }
+
+template <int DT, bool SWIGLU, int XDT>
+int vector_launch(const Int8Args& a, hipStream_t st) {
+  static std::atomic<uint64_t> set{0};  // GPUs on which the kernel may take its shared memory
+  int dev = -1;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return MQ_ERR_LAUNCH;
+  if (!(set.load() >> dev & 1)) {
+    if (hipFuncSetAttribute((const void*)int8_vector_kernel<DT, SWIGLU, XDT>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                            160 * 1024) != hipSuccess)
+      return MQ_ERR_LAUNCH;
+    set.fetch_or(1ull << dev);
+  }
+  const int pairs = SWIGLU ? a.N : (a.N + 1) / 2, waves = VEC_THREADS / 64;
+  // 512 workgroups, two a CU, walk over what they do not reach at once: 26 us at 18432 x 7168 (5.1 TB/s) against 32 with 256
+  // of them and 30 with 2048; 6.3 us at 2048 x 7168 (256 workgroups)
+  const int gx = min((pairs + waves - 1) / waves, 512);
+  hipLaunchKernelGGL((int8_vector_kernel<DT, SWIGLU, XDT>), dim3(gx), dim3(VEC_THREADS),
+                     vector_smem(a.K), st, a);
+  return mq_check_launch();
+}
+
+bool rows_of_words(const int8_t* p, long ld) { return ((uintptr_t)p & 3) == 0 && ld % 4 == 0; }
+
+// the vector kernel takes one or two rows whose codes fit its shared memory
+bool for_vector(int M, int K) { return M <= VT && K >= 16 && vector_smem(K) <= 160 * 1024; }
+// plain products with this many 256 x 256 tiles or more go to the tiles: measured 49 against 74 us at 1024 x 7168 x 2048 (112
+// tiles), 36 against 29 at 1024 x 4096 x 1024 (64)
+bool enough_tiles(int M, int N, int swiglu) {
+  return ((long)M + TM - 1) / TM * (((long)N * (swiglu ? 2 : 1) + TN - 1) / TN) >= 80;
+}
+
+template <int DT, bool SWIGLU>
+int int8_launch(const Int8Args& a, hipStream_t st) {
+  const bool tiles = a.K >= 16 && rows_of_words(a.A, a.lda) && rows_of_words(a.B, a.ldb) && a.strideB % 4 == 0;
+  if (a.offsets) {
+    // up to four rows an expert on average the weights' bytes decide: 203 + 121 us against 222 + 134 with 128 rows over 64
+    // experts of 7168 x 2048; with 512 rows the tiles win, 325 + 210 against 391 + 214
+    if (!tiles || a.M <= 4l * a.E) return thin_launch<DT, SWIGLU, 2, 2, 2>(a, st);
+    return tile_launch<DT, SWIGLU>(a, st);
+  }
+  if (for_vector(a.M, a.K)) return vector_launch<DT, SWIGLU, -1>(a, st);
+  if (tiles && enough_tiles(a.M, a.N, SWIGLU)) return tile_launch<DT, SWIGLU>(a, st);
+  // the largest block of results that still gives 192 workgroups
+  const auto groups = [&](int R, int C) {
+    const int outn = SWIGLU ? 8 * C : 16 * C;
+    return (long)((a.M + 16 * R - 1) / (16 * R)) * ((a.N + outn - 1) / outn);
+  };
+  if (groups(4, 4) >= 192) return thin_launch<DT, SWIGLU, 4, 4, 1>(a, st);  // 38 us at 512 x 4096 x 4096, (2, 4) 53, (2, 2) 62
+  if (groups(2, 4) >= 192) return thin_launch<DT, SWIGLU, 2, 4, 4>(a, st);  // 9.3 us at 256 x 2048 x 2048, (4, 4) 12, (2, 2) 11
+  if (groups(2, 2) >= 192) return thin_launch<DT, SWIGLU, 2, 2, 2>(a, st);  // 16 us at 333 x 576 x 7168, (4, 4) 30, (1, 1) 23
+  if (groups(1, 2) >= 192 || SWIGLU) return thin_launch<DT, SWIGLU, 1, 2, 2>(a, st);  // 42 us at 16 x 18432 x 7168, (1, 1) 45
+  return thin_launch<DT, SWIGLU, 1, SWIGLU ? 2 : 1, 4>(a, st);  // 8.6 us at 8 x 2048 x 7168, (1, 2) 11
+}
+
+// Rows that start at any byte, copied to rows that start at multiples of 16 (for the tiles).
+__global__ __launch_bounds__(256) void align_rows_kernel(const int8_t* __restrict__ from, long ld, int K, int8_t* __restrict__ to,
+                                                         long ldt) {
+  const int8_t* p = from + (long)blockIdx.x * ld;
+  int8_t* q = to + (long)blockIdx.x * ldt;
+  for (int c = threadIdx.x * 16; c < K; c += 256 * 16) {
+    if (c + 16 <= K) {
+      intx4 v;
+      __builtin_memcpy(&v, p + c, 16);
+      *reinterpret_cast<intx4*>(q + c) = v;
+    } else {
+      for (int i = c; i < K; ++i) q[i] = p[i];
+    }
+  }
+}
+
+size_t padded(int K) { return ((size_t)K + 15) / 16 * 16; }
+// K no multiple of 4: contiguous rows start anywhere; large products copy them first (30 us for 8192 x 7781 weights against
+// the millisecond that such rows cost a product of 4096 tokens)
+bool aligns_rows(int M, int N, int K, int swiglu) { return K % 4 != 0 && K >= 16 && enough_tiles(M, N, swiglu); }
+
+int int8_dispatch(Int8Args a, int dtype, int swiglu, int8_t* ws, hipStream_t st) {
+  if (ws && aligns_rows(a.M, a.N, a.K, swiglu)) {
+    const long ld = (long)padded(a.K);
+    const int rows_b = swiglu ? 2 * a.N : a.N;
+    if (!rows_of_words(a.B, a.ldb)) {
+      hipLaunchKernelGGL(align_rows_kernel, dim3(rows_b), dim3(256), 0, st, a.B, a.ldb, a.K, ws, ld);
+      a.B = ws;
+      a.ldb = ld;
+    }
+    if (!rows_of_words(a.A, a.lda)) {
+      int8_t* to = ws + (size_t)rows_b * ld;
+      hipLaunchKernelGGL(align_rows_kernel, dim3(a.M), dim3(256), 0, st, a.A, a.lda, a.K, to, ld);
+      a.A = to;
+      a.lda = ld;
+    }
+  }
   // runs of four results leave in one store where rows of Y allow it
   const int run = dtype == DT_F32 ? 16 : 8;
   a.vec_out = a.N % 4 == 0 && ((uintptr_t)a.Y % run) == 0 && a.ldy % 4 == 0;
   if (dtype == DT_F32) return swiglu ? int8_launch<DT_F32, true>(a, st) : int8_launch<DT_F32, false>(a, st);
   if (dtype == DT_BF16) return swiglu ? int8_launch<DT_BF16, true>(a, st) : int8_launch<DT_BF16, false>(a, st);
   return swiglu ? int8_launch<DT_F16, true>(a, st) : int8_launch<DT_F16, false>(a, st);
+}
+
+bool is_dtype(int d) { return d == DT_F32 || d == DT_BF16 || d == DT_F16; }
+
+void quantize(const void* X, int dtype, long ldx, int n, int C, int8_t* Q, long ldq, float* scale, hipStream_t st) {
+  if (dtype == DT_F32) quantize_launch<DT_F32>(X, ldx, n, C, Q, ldq, scale, st);
+  else if (dtype == DT_BF16) quantize_launch<DT_BF16>(X, ldx, n, C, Q, ldq, scale, st);
+  else quantize_launch<DT_F16>(X, ldx, n, C, Q, ldq, scale, st);
 }
 
 constexpr int MAX_K = 131071;  // |sum| <= K 128 128 stays inside 32 bits
@@ -788,27 +1019,29 @@ constexpr int MAX_K = 131071;  // |sum| <= K 128 128 stays inside 32 bits
 extern "C" int mq_quantize_tokens(const void* X, int dtype, long ldx, int n, int C, int8_t* Q, long ldq, float* scale,
                                   void* stream) {
   if (n < 0 || C <= 0 || ldx < C || ldq < C) return MQ_ERR_ARG;
-  if (dtype != DT_F32 && dtype != DT_BF16 && dtype != DT_F16) return MQ_ERR_ARG;
+  if (!is_dtype(dtype)) return MQ_ERR_ARG;
   if (n == 0) return MQ_OK;
   if (!X || !Q || !scale) return MQ_ERR_ARG;
-  hipStream_t st = (hipStream_t)stream;
-  if (dtype == DT_F32) quantize_launch<DT_F32>(X, ldx, n, C, Q, ldq, scale, st);
-  else if (dtype == DT_BF16) quantize_launch<DT_BF16>(X, ldx, n, C, Q, ldq, scale, st);
-  else quantize_launch<DT_F16>(X, ldx, n, C, Q, ldq, scale, st);
+  quantize(X, dtype, ldx, n, C, Q, ldq, scale, (hipStream_t)stream);
   return mq_check_launch();
 }
 
-extern "C" size_t mq_matmul_int8_workspace_bytes(int M, int N, int K, int swiglu) { return 0; }
+extern "C" size_t mq_matmul_int8_workspace_bytes(int M, int N, int K, int swiglu) {
+  if (M <= 0 || N <= 0 || K <= 0 || !aligns_rows(M, N, K, swiglu)) return 0;
+  return ((size_t)M + (size_t)N * (swiglu ? 2 : 1)) * padded(K);
+}
 
 extern "C" int mq_matmul_int8(const int8_t* A, long lda, const float* a_scale, const int8_t* B, long ldb,
                               const float* b_scale, const void* bias, void* Y, long ldy, int out_dtype, int M, int N, int K,
                               int swiglu, void* workspace, size_t workspace_bytes, void* stream) {
   if (M < 0 || N <= 0 || K <= 0 || K > MAX_K || lda < K || ldb < K || ldy < N || (swiglu && bias)) return MQ_ERR_ARG;
-  if (out_dtype != DT_F32 && out_dtype != DT_BF16 && out_dtype != DT_F16) return MQ_ERR_ARG;
+  if (!is_dtype(out_dtype)) return MQ_ERR_ARG;
   if (M == 0) return MQ_OK;
   if (!A || !a_scale || !B || !b_scale || !Y) return MQ_ERR_ARG;
+  const size_t need = mq_matmul_int8_workspace_bytes(M, N, K, swiglu);
+  if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) return MQ_ERR_WORKSPACE;
   const Int8Args a = {A, lda, a_scale, nullptr, M, B, ldb, 0, b_scale, bias, Y, ldy, M, N, K, nullptr, 1, 0};
-  return int8_dispatch(a, out_dtype, swiglu, (hipStream_t)stream);
+  return int8_dispatch(a, out_dtype, swiglu, need ? (int8_t*)workspace : nullptr, (hipStream_t)stream);
 }
 
 extern "C" int mq_matmul_int8_grouped(const int8_t* A, long lda, const float* a_scale, int src_rows, const long* rows, int S,
@@ -817,9 +1050,40 @@ extern "C" int mq_matmul_int8_grouped(const int8_t* A, long lda, const float* a_
                                       void* stream) {
   if (S < 0 || E <= 0 || E > 1024 || N <= 0 || K <= 0 || K > MAX_K || lda < K || ldb < K || ldy < N) return MQ_ERR_ARG;
   if (src_rows < 0 || strideB < 0 || (!rows && src_rows < S)) return MQ_ERR_ARG;
-  if (out_dtype != DT_F32 && out_dtype != DT_BF16 && out_dtype != DT_F16) return MQ_ERR_ARG;
+  if (!is_dtype(out_dtype)) return MQ_ERR_ARG;
   if (S == 0) return MQ_OK;
   if (!A || !a_scale || !B || !b_scale || !offsets || !Y) return MQ_ERR_ARG;
   const Int8Args a = {A, lda, a_scale, rows, src_rows, B, ldb, strideB, b_scale, nullptr, Y, ldy, S, N, K, offsets, E, 0};
-  return int8_dispatch(a, out_dtype, swiglu, (hipStream_t)stream);
+  return int8_dispatch(a, out_dtype, swiglu, nullptr, (hipStream_t)stream);
+}
+
+extern "C" size_t mq_linear_int8_workspace_bytes(int M, int N, int K) {
+  if (M <= 0 || N <= 0 || K <= 0 || for_vector(M, K)) return 0;
+  const size_t tokens = (size_t)M * padded(K) + ((size_t)M * sizeof(float) + 15) / 16 * 16;
+  return tokens + (aligns_rows(M, N, K, 0) ? (size_t)N * padded(K) : 0);
+}
+
+extern "C" int mq_linear_int8(const void* X, int dtype, long ldx, const int8_t* B, long ldb, const float* b_scale,
+                              const void* bias, void* Y, long ldy, int M, int N, int K, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  if (M < 0 || N <= 0 || K <= 0 || K > MAX_K || ldx < K || ldb < K || ldy < N || !is_dtype(dtype)) return MQ_ERR_ARG;
+  if (M == 0) return MQ_OK;
+  if (!X || !B || !b_scale || !Y) return MQ_ERR_ARG;
+  hipStream_t st = (hipStream_t)stream;
+  Int8Args a = {(const int8_t*)X, ldx, nullptr, nullptr, M, B, ldb, 0, b_scale, bias, Y, ldy, M, N, K, nullptr, 1, 0};
+  if (for_vector(M, K)) {  // one launch: every workgroup quantizes the row or two for itself
+    if (dtype == DT_F32) return vector_launch<DT_F32, false, DT_F32>(a, st);
+    if (dtype == DT_BF16) return vector_launch<DT_BF16, false, DT_BF16>(a, st);
+    return vector_launch<DT_F16, false, DT_F16>(a, st);
+  }
+  const size_t need = mq_linear_int8_workspace_bytes(M, N, K);
+  if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)) return MQ_ERR_WORKSPACE;
+  float* scale = reinterpret_cast<float*>(workspace);
+  int8_t* codes = reinterpret_cast<int8_t*>(workspace) + ((size_t)M * sizeof(float) + 15) / 16 * 16;
+  int8_t* rest = codes + (size_t)M * padded(K);
+  quantize(X, dtype, ldx, M, K, codes, (long)padded(K), scale, st);
+  a.A = codes;
+  a.lda = (long)padded(K);
+  a.sa = scale;
+  return int8_dispatch(a, dtype, 0, rest, st);
 }

@@ -803,6 +803,32 @@ def matmul_int8(A: Tensor, a_scale: Tensor, B: Tensor, b_scale: Tensor, bias: Op
     return Y
 
 
+def linear_int8(X: Tensor, B: Tensor, b_scale: Tensor, bias: Optional[Tensor] = None) -> Tensor:
+    """`matmul_int8(*quantize_tokens(X), B, b_scale, bias, X.dtype)` in one call, and in one launch for one or two rows:
+    X (M, K) fp32/bf16/fp16, B (N, K) int8 with b_scale (N,) fp32, bias (N,) of X's type."""
+    if X.dim() != 2 or X.dtype not in _DT:
+        raise ValueError("X must be (M, K) fp32, bf16 or fp16")
+    K = X.shape[1]
+    if B.dim() != 2 or B.dtype != torch.int8 or B.shape[1] != K or not 1 <= K <= _MAX_K or B.shape[0] < 1:
+        raise ValueError(f"B must be (N, K) int8 with X's K columns, 1 <= K <= {_MAX_K}")
+    N = B.shape[0]
+    if b_scale.dtype != torch.float32 or b_scale.shape != (N,) or not b_scale.is_contiguous():
+        raise ValueError("b_scale must be contiguous fp32, one value per row of B")
+    if bias is not None and (bias.dtype != X.dtype or bias.shape != (N,) or not bias.is_contiguous()):
+        raise ValueError("bias must be a contiguous vector of X's type with one value per row of B")
+    with _on(X, B, b_scale, bias):
+        (X, ldx), (B, ldb) = _rows(X), _rows(B)
+        M = X.shape[0]
+        lib = _lib.load()
+        Y = torch.empty(M, N, dtype=X.dtype, device=X.device)
+        need = lib.mq_linear_int8_workspace_bytes(M, N, K)
+        ws = torch.empty(need, dtype=torch.uint8, device=X.device) if need else None
+        rc = lib.mq_linear_int8(X.data_ptr(), _DT[X.dtype], ldx, B.data_ptr(), ldb, b_scale.data_ptr(), _p(bias), Y.data_ptr(),
+                                N, M, N, K, _p(ws), need, _stream(X))
+    check(rc, "mq_linear_int8")
+    return Y
+
+
 def matmul_int8_grouped(A: Tensor, a_scale: Tensor, B: Tensor, b_scale: Tensor, offsets: Tensor,
                         rows: Optional[Tensor] = None, out_dtype: torch.dtype = torch.bfloat16, swiglu: bool = False,
                         out: Optional[Tensor] = None) -> Tensor:

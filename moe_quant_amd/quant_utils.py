@@ -127,8 +127,9 @@ def linear_int8(x: Tensor, weight: Tensor, weight_scale: Tensor, bias: Optional[
     every token is quantized to 8 bits with a scale of its own on the way in.  Returns (..., R) of x's type."""
     if x.dim() < 1:
         raise ValueError("x must be (..., C)")
-    codes, scale = ops.quantize_tokens(x.reshape(-1, x.shape[-1]))
-    return ops.matmul_int8(codes, scale, weight, weight_scale, bias, x.dtype).view(*x.shape[:-1], weight.shape[0])
+    if x.dim() == 2:
+        return ops.linear_int8(x, weight, weight_scale, bias)
+    return ops.linear_int8(x.reshape(-1, x.shape[-1]), weight, weight_scale, bias).view(*x.shape[:-1], weight.shape[0])
 
 
 def get_relative_mse_error(q: Tensor, w: Tensor, H: Optional[Tensor] = None):

@@ -345,7 +345,7 @@ SHAPES = [(1, 1, 1), (1, 2048, 7168), (1, 7, 33), (2, 64, 64), (3, 100, 500), (4
           (16, 256, 256), (17, 257, 255), (31, 40, 1000), (33, 576, 7168), (64, 192, 96), (65, 129, 640), (100, 1536, 320),
           (127, 128, 64), (128, 128, 128), (129, 384, 192), (255, 255, 257), (256, 256, 128), (257, 300, 384), (300, 1000, 72),
           (333, 576, 7168), (512, 520, 208), (700, 2048, 48), (1025, 264, 1040), (2, 5000, 16), (60, 33, 16400),
-          (320, 320, 16)]
+          (320, 320, 16), (4100, 4200, 64), (2100, 2600, 130), (2561, 2304, 449), (1500, 5000, 20)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
@@ -399,9 +399,51 @@ def test_product_views(dev, M):
     assert ops.matmul_int8(A.to(dev)[:0], sa.to(dev)[:0], B.to(dev), sb.to(dev)).shape == (0, 260)
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 2048, 7168), (1, 1, 16), (1, 33, 1000), (2, 70, 1003), (2, 576, 17), (1, 9, 5), (3, 100, 257),
+                                   (1, 40, 81920), (2, 24, 90001), (17, 64, 300), (300, 520, 130), (2100, 2600, 133), (2048, 2560, 96)])
+def test_linear_equals_its_two_halves(dev, M, N, K):
+    """quantize + product in one call: the same bits as the two calls (and their exact codes, for the fused rows too)."""
+    g = _gen(M + N + K)
+    B, sb = _rand_codes(g, N, K), (torch.rand(N, generator=g) + 0.1) / (100 * K**0.5)
+    for name, dt in DT.items():
+        _say("linear", M, N, K, name)
+        x = torch.randn(M, K, generator=g)
+        x[:, K // 3] *= 20
+        x[-1, K // 2:] = 0 if M > 1 else x[-1, K // 2:]
+        x = x.to(dt)
+        bias = torch.randn(N, generator=g).to(dt)
+        for b in (None, bias.to(dev)):
+            got = ops.linear_int8(x.to(dev), B.to(dev), sb.to(dev), b)
+            q, s = ops.quantize_tokens(x.to(dev))
+            assert torch.equal(got, ops.matmul_int8(q, s, B.to(dev), sb.to(dev), b, dt))
+        q, s = _codes64(x)
+        want, mag, _ = _product64(q, s, B, sb, bias)
+        _close(got, want, mag * (1 + U), None, dt)
+
+
+def test_linear_special_rows(dev):
+    """Rows of zeros, with a NaN, an infinity, and tiny ones, one and many tokens at a time."""
+    g = _gen(77)
+    B, sb = _rand_codes(g, 50, 300).to(dev), torch.ones(50, device=dev)
+    x = torch.randn(5, 300, generator=g)
+    x[0], x[1, 9], x[2, 299] = 0, math.nan, -math.inf
+    x[3] *= 2.0**-120
+    x = x.to(dev)
+    whole = ops.linear_int8(x, B, sb)
+    assert (whole[0] == 0).all() and whole[1:3].isnan().all() and whole[3:].isfinite().all()
+    for r in range(5):
+        for n in (1, 2):
+            got = ops.linear_int8(x[r:r + n], B, sb)
+            assert torch.equal(got.nan_to_num(7), whole[r:r + n].nan_to_num(7))
+    assert ops.linear_int8(x[:0], B, sb).shape == (0, 50)
+    y = ops.linear_int8(x.t()[:, :3].t(), B, sb)  # another stride
+    assert torch.equal(y.nan_to_num(7), whole[:3].nan_to_num(7))
+
+
 GROUPS = [([5], 40, 64), ([0, 0, 3], 130, 96), ([1] * 9, 64, 512), ([16, 0, 17, 1, 33], 96, 256), ([130, 0, 64, 1], 200, 128),
           ([300, 5, 0, 257], 264, 320), ([2, 1, 0, 0, 4, 0, 0], 576, 1030), ([700], 300, 144), ([0, 0], 32, 32),
-          ([128, 128, 256], 512, 192), ([1] * 70, 48, 80), ([3] * 200, 16, 48)]
+          ([128, 128, 256], 512, 192), ([1] * 70, 48, 80), ([3] * 200, 16, 48), ([600, 256, 0, 513, 77], 9000, 64), ([255, 33, 97, 129], 5200, 452),
+          ([40, 70, 0, 300], 64, 10)]
 
 
 @pytest.mark.parametrize("counts,N,K", GROUPS)

@@ -76,6 +76,15 @@ def test_product_refusals():
     for bad in (torch.zeros(3), torch.zeros(3, 4, dtype=torch.float64), torch.zeros(3, 0)):
         with pytest.raises(ValueError):
             ops.quantize_tokens(bad)
+    x = torch.zeros(3, 32)
+    for bad in ((x[0], B, sb), (x.double(), B, sb), (x[:, :31], B, sb), (x, B.short(), sb), (x, B[None], sb), (x, B, sb[:5]),
+                (x, B, sb.double()), (x, B, sb, torch.zeros(5)), (x, B, sb, torch.zeros(6).half()), (x[:, :0], B[:, :0], sb)):
+        with pytest.raises(ValueError):
+            ops.linear_int8(*bad)
+    with pytest.raises(ValueError):
+        quant_utils.linear_int8(torch.zeros(()), B, sb)
+    with pytest.raises(_lib.MoeQuantHipError):
+        quant_utils.linear_int8(x, B, sb)
 
 
 def test_grouped_refusals():
@@ -135,6 +144,21 @@ def test_c_abi_refusals():
                 dict(K=131072, lda=131072, ldb=131072), dict(sw=1, bias=p)):
         assert product(**bad) == ARG, bad
     assert product(M=0) == _lib.MQ_OK
+
+    def linear(**k):
+        a = dict(X=p, dt=1, ldx=32, B=p, ldb=32, sb=p, bias=None, Y=p, ldy=8, M=4, N=8, K=32, ws=p, wsb=4096)
+        a.update(k)
+        return lib.mq_linear_int8(*a.values(), None)
+
+    for bad in (dict(X=None), dict(ldx=31), dict(ldb=31), dict(ldy=7), dict(dt=-1), dict(N=0), dict(K=0), dict(M=-1), dict(Y=None),
+                dict(K=131072, ldx=131072, ldb=131072)):
+        assert linear(**bad) == ARG, bad
+    need = lib.mq_linear_int8_workspace_bytes(4, 8, 32)
+    assert need == 4 * 32 + 16 and lib.mq_linear_int8_workspace_bytes(1, 8, 32) == 0 and linear(M=0) == _lib.MQ_OK
+    assert linear(ws=None) == WS and linear(wsb=need - 1) == WS
+    odd = lib.mq_matmul_int8_workspace_bytes(4096, 4096, 1001, 0)
+    assert odd == 8192 * 1008 and lib.mq_matmul_int8_workspace_bytes(4096, 4096, 1004, 0) == 0
+    assert product(M=4096, N=4096, K=1001, lda=1001, ldb=1001, ldy=4096) == WS
 
     def grouped(**k):
         a = dict(A=p, lda=32, sa=p, src=4, rows=None, S=4, B=p, ldb=32, st=256, sb=p, E=2, off=p, Y=p, ldy=8, dt=1, N=8, K=32, sw=0)
