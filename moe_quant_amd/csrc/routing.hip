@@ -59,24 +59,47 @@ __global__ __launch_bounds__(256) void sort_scan_kernel(int* __restrict__ count,
   if (threadIdx.x == 0) total[blockIdx.x] = base;
 }
 
-// ALONE: one workgroup does the whole sort (n <= SORT_CHUNK) and counts for itself.
+// n / k for 0 <= n < 2^31, k >= 1: with 2^(s-1) < k <= 2^s and mul = ceil(2^(31+s) / k) < 2^32 the quotient is
+// n mul >> (31 + s), as mul exceeds 2^(31+s) / k by less than 2^s / k <= 2^(31+s) / (k n)
+struct Divider {
+  uint32_t mul;
+  int shift;  // s - 1; k = 1: -1
+  static Divider of(int k) {
+    int s = 0;
+    while ((1l << s) < k) ++s;
+    if (s == 0) return {0, -1};
+    return {(uint32_t)(((1ul << (31 + s)) + k - 1) / k), s - 1};
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return shift < 0 ? n : __umulhi(n, mul) >> shift; }
+};
+
+// A wavefront ranks its run of choices 64 at a time: the lanes that hold the same bin are found by a ballot a bit of the bin
+// (stable: a lane's rank is the number of such lanes before it), then the bin's next position moves on.  The choices stay
+// in registers between counting and ranking.  ALONE: one workgroup does the whole sort (n <= SORT_CHUNK) and counts for
+// itself.
 template <bool ALONE>
-__global__ __launch_bounds__(512) void sort_scatter_kernel(const long* __restrict__ ids, int n, int k, int E, int blocks,
-                                                           const int* __restrict__ count, const int* __restrict__ total,
-                                                           long* __restrict__ rows, long* __restrict__ offsets,
-                                                           int* __restrict__ slots) {
+__global__ __launch_bounds__(512) void sort_scatter_kernel(const long* __restrict__ ids, int n, Divider k, int E, int bits,
+                                                           int blocks, const int* __restrict__ count,
+                                                           const int* __restrict__ total, long* __restrict__ rows,
+                                                           long* __restrict__ offsets, int* __restrict__ slots) {
   __shared__ int pos[SORT_WAVES][SORT_MAX_E + 1];  // choices of a bin in a wavefront's run, then its next position
   __shared__ int start[SORT_MAX_E + 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int STEPS = SORT_CHUNK / SORT_WAVES / 64;
+  const int steps = ALONE ? ((n + SORT_WAVES - 1) / SORT_WAVES + 63) / 64 : STEPS;
+  const int i0 = (int)blockIdx.x * SORT_CHUNK + wave * steps * 64;
+  int bin[STEPS];
+#pragma unroll
+  for (int q = 0; q < STEPS; ++q) {
+    const int i = i0 + q * 64 + lane;
+    bin[q] = q < steps && i < n ? bin_of(ids[i], E) : E + 1;
+  }
   for (int w = 0; w < SORT_WAVES; ++w)
     for (int b = threadIdx.x; b <= E; b += 512) pos[w][b] = 0;
   __syncthreads();
-  const int per = ALONE ? ((n + SORT_WAVES - 1) / SORT_WAVES + 63) / 64 * 64 : SORT_CHUNK / SORT_WAVES;
-  const long i0 = (long)blockIdx.x * SORT_CHUNK + wave * per;
-  for (int q = 0; q < per; q += 64) {
-    const long i = i0 + q + lane;
-    if (i < n) atomicAdd(&pos[wave][bin_of(ids[i], E)], 1);
-  }
+#pragma unroll
+  for (int q = 0; q < STEPS; ++q)
+    if (bin[q] <= E) atomicAdd(&pos[wave][bin[q]], 1);
   __syncthreads();
   if (wave == 0) {  // exclusive prefix of the bins' totals
     int base = 0;
@@ -84,9 +107,12 @@ __global__ __launch_bounds__(512) void sort_scatter_kernel(const long* __restric
       const int b = b0 + lane;
       int v = 0;
       if (b <= E) {
-        if (ALONE)
+        if (ALONE) {
+#pragma unroll
           for (int w = 0; w < SORT_WAVES; ++w) v += pos[w][b];
-        else v = total[b];
+        } else {
+          v = total[b];
+        }
       }
       int s = v;
       for (int o = 1; o < 64; o <<= 1) {
@@ -101,6 +127,7 @@ __global__ __launch_bounds__(512) void sort_scatter_kernel(const long* __restric
   for (int b = threadIdx.x; b <= E; b += 512) {
     int at = start[b] + (ALONE ? 0 : count[(long)b * blocks + blockIdx.x]);
     if (blockIdx.x == 0) offsets[b] = start[b];
+#pragma unroll
     for (int w = 0; w < SORT_WAVES; ++w) {
       const int c = pos[w][b];
       pos[w][b] = at;
@@ -108,23 +135,26 @@ __global__ __launch_bounds__(512) void sort_scatter_kernel(const long* __restric
     }
   }
   __syncthreads();
-  for (int q = 0; q < per; q += 64) {
-    const long i = i0 + q + lane;
-    const bool in = i < n;
-    const int b = in ? bin_of(ids[i], E) : E + 1;
-    unsigned long same = ~0ul;  // lanes with this lane's bin
-    for (int bit = 0; bit < 11; ++bit) {
+#pragma unroll
+  for (int q = 0; q < STEPS; ++q) {
+    if (q >= steps) break;
+    const int b = bin[q], i = i0 + q * 64 + lane;
+    const bool in = b <= E;
+    uint32_t lo = ~0u, hi = ~0u;  // lanes with this lane's bin
+    for (int bit = 0; bit < bits; ++bit) {
       const unsigned long set = __ballot(b >> bit & 1);
-      same &= (b >> bit & 1) ? set : ~set;
+      const uint32_t flip = (b >> bit & 1) - 1;
+      lo &= (uint32_t)set ^ flip;
+      hi &= (uint32_t)(set >> 32) ^ flip;
     }
-    const int before = __popcll(same & ((1ul << lane) - 1));
+    const int before = __builtin_amdgcn_mbcnt_hi(hi, __builtin_amdgcn_mbcnt_lo(lo, 0));
     if (in) {
       const int at = pos[wave][b] + before;
-      rows[at] = i / k;
+      rows[at] = k.div(i);
       if (slots) slots[i] = b == E ? -1 : at;
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (in && before == 0) pos[wave][b] += __popcll(same);
+    if (in && before == 0) pos[wave][b] += __popc(lo) + __popc(hi);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 }
@@ -213,8 +243,11 @@ extern "C" int mq_sort_by_expert(const long* ids, int T, int top_k, int E, long*
   if (!offsets || (T > 0 && (!ids || !rows))) return MQ_ERR_ARG;
   hipStream_t st = (hipStream_t)stream;
   const int n = T * top_k;
+  const Divider k = Divider::of(top_k);
+  int bits = 0;
+  while ((E + 1) >> bits) ++bits;
   if (n <= SORT_CHUNK) {
-    hipLaunchKernelGGL((sort_scatter_kernel<true>), dim3(1), dim3(512), 0, st, ids, n, top_k, E, 1, nullptr, nullptr, rows,
+    hipLaunchKernelGGL((sort_scatter_kernel<true>), dim3(1), dim3(512), 0, st, ids, n, k, E, bits, 1, nullptr, nullptr, rows,
                        offsets, slots);
     return mq_check_launch();
   }
@@ -224,7 +257,7 @@ extern "C" int mq_sort_by_expert(const long* ids, int T, int top_k, int E, long*
   int* count = total + E + 1;
   hipLaunchKernelGGL(sort_count_kernel, dim3(blocks), dim3(512), 0, st, ids, n, E, blocks, count);
   hipLaunchKernelGGL(sort_scan_kernel, dim3(E + 1), dim3(256), 0, st, count, blocks, total);
-  hipLaunchKernelGGL((sort_scatter_kernel<false>), dim3(blocks), dim3(512), 0, st, ids, n, top_k, E, blocks, count, total,
+  hipLaunchKernelGGL((sort_scatter_kernel<false>), dim3(blocks), dim3(512), 0, st, ids, n, k, E, bits, blocks, count, total,
                      rows, offsets, slots);
   return mq_check_launch();
 }
