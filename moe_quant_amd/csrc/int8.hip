@@ -187,7 +187,7 @@ struct Int8Args {
   int M, N, K;  // N: columns of Y
   const long* offsets;  // grouped: expert e owns rows offsets[e] .. offsets[e + 1)
   int E;
-  int vec_out;
+  int vec_out;  // runs of four results may be stored at once; 2: of eight
 };
 
 // four results of one row, columns n .. n + 3, as far as they exist
@@ -245,6 +245,8 @@ struct TileShared {
                                // of this one and of the next
   int full[MAX_GROUPS + 64], part[MAX_GROUPS + 64];  // whole tiles and partly filled ones before expert e
   int lo[MAX_GROUPS], hi[MAX_GROUPS];
+  float scale[2][8][64];  // this tile's (a slow wavefront may still use the last one's): a wavefront loads 32 columns' and 32 rows'
+  float bias[2][TN];
 };
 static_assert(sizeof(TileShared) <= 160 * 1024, "shared memory of a CU");
 
@@ -268,6 +270,8 @@ __device__ __forceinline__ void load_lds4(const void* p, unsigned lds_addr) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(lds_addr) : "memory", "m0");
 }
 
+static __device__ const float no_scale = 0.f;  // of a row that is none
+
 struct Job {
   int e, m0, mend, n0;
 };
@@ -281,7 +285,7 @@ struct TileKernel {
   const int nk;         // stages of a tile
   const int chunk;      // this lane's chunk of a stage's 64 bytes in direct loads
   const unsigned lds0;  // LDS address of the stages
-  const unsigned rows0;
+  const unsigned rows0, scale0;
   intx16 acc[4][2];
   intx4 fa0[4], fb0[2];
   const int8_t *src[4], *next[4];
@@ -293,7 +297,8 @@ struct TileKernel {
   __device__ __forceinline__ TileKernel(const Int8Args& args, TileShared& s)
       : a(args), sh(s), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), wm(wave >> 2),
         wn(wave & 3), lr(lane & 31), lk(lane >> 5), nk(max((args.K + TK - 1) / TK, MIN_STAGES)),
-        chunk((lane & 3) ^ (lane >> 4)), lds0(lds_of(&s.stage[0][0])), rows0(lds_of(&s.rows[0][0])), slot(0) {}
+        chunk((lane & 3) ^ (lane >> 4)), lds0(lds_of(&s.stage[0][0])), rows0(lds_of(&s.rows[0][0])), scale0(lds_of(&s.scale[0][0][0])),
+        slot(0) {}
 
   // Experts' ranges (clamped to [0, M]; a plain product is one expert's) and the whole and partly filled row tiles before
   // each; returns how many there are of both.
@@ -451,32 +456,68 @@ struct TileKernel {
     }
   }
 
-  __device__ __forceinline__ void results(const Job& j, int buf) const {
+  // Scales of a tile on their way to shared memory: lane 0..31 a column's, 32..63 a row's (SwiGLU: 16 gate columns', the same
+  // 16 up columns', 32 rows').  Loaded while the tile is computed: 32 waits for memory in its epilogue cost 25 us a tile.
+  __device__ __forceinline__ void load_scales(const Job& j, int buf, int half) {
     const float* sb = a.sb + (long)j.e * (SWIGLU ? 2 * a.N : a.N);
+    const int l = lane & 31, r = 32 * wave + l;
+    const float* p;
+    if (lane < 32) {
+      const int col = min(j.n0 + (SWIGLU ? 16 * wave + (l & 15) : r), a.N - 1);
+      p = sb + (SWIGLU && l >= 16 ? a.N + col : col);
+    } else {
+      const long from = a.rows ? sh.rows[buf][r] : min(j.m0 + r, j.mend - 1);
+      p = from >= 0 && from < a.src_rows ? a.sa + from : &no_scale;
+    }
+    load_lds4(p, scale0 + (unsigned)(half * 8 + wave) * 256u);
+    if (!SWIGLU && a.bias && threadIdx.x < TN) sh.bias[half][threadIdx.x] = load_val<DT>(a.bias, min(j.n0 + (int)threadIdx.x, a.N - 1));
+  }
+
+  __device__ __forceinline__ void results(const Job& j, int half) const {
+    constexpr int RUNS = SWIGLU ? 4 : 8;  // of four columns: 8 g + 4 lk of the wavefront's 32-column blocks
+    const int first = j.n0 + (SWIGLU ? wn * 32 : wn * 64) + 4 * lk;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int r = wm * 128 + i * 32 + lr, m = j.m0 + r;
-      if (m >= j.mend) continue;
-      const long from = a.rows ? sh.rows[buf][r] : m;
-      const float sa = from >= 0 && from < a.src_rows ? a.sa[from] : 0.f;
+      const int m = j.m0 + wm * 128 + i * 32 + lr;
+      const float sa = sh.scale[half][wm * 4 + i][32 + lr];
+      const bool in = m < j.mend;
+      const long row = (long)m * a.ldy;
 #pragma unroll
-      for (int c0 = 0; c0 < (SWIGLU ? 1 : 2); ++c0)
+      for (int g = 0; g < RUNS; g += 2) {
+        float y[2][4];
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int n = j.n0 + (SWIGLU ? wn * 32 : wn * 64 + c0 * 32) + 8 * g + 4 * lk;
-          float y[4];
+        for (int h = 0; h < 2; ++h) {
+          const int c = (g + h) * 8 + 4 * lk;  // in the wavefront's 32 (SwiGLU) or 64 columns
+          const float* s0 = SWIGLU ? &sh.scale[half][wn * 2 + (c >> 4)][c & 15] : &sh.scale[half][wn * 2 + (c >> 5)][c & 31];
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
-            const int c = min(n + v, a.N - 1);
             if (SWIGLU) {
-              y[v] = silu_times((float)acc[i][0][4 * g + v] * sa * sb[c], (float)acc[i][1][4 * g + v] * sa * sb[a.N + c]);
+              y[h][v] = silu_times((float)acc[i][0][4 * (g + h) + v] * sa * s0[v], (float)acc[i][1][4 * (g + h) + v] * sa * s0[16 + v]);
             } else {
-              y[v] = (float)acc[i][c0][4 * g + v] * sa * sb[c];
-              if (a.bias) y[v] += load_val<DT>(a.bias, c);
+              y[h][v] = (float)acc[i][(g + h) >> 2][4 * ((g + h) & 3) + v] * sa * s0[v];
+              if (a.bias) y[h][v] += sh.bias[half][wn * 64 + c + v];
             }
           }
-          store_run<DT>(a.Y, (long)m * a.ldy, n, a.N, a.vec_out, y);
         }
+        if (DT != DT_F32 && a.vec_out == 2) {
+          // lanes l and l + 32 hold columns 8 g .. + 3 and + 4 .. + 7 of one row, and the same of the next run: they swap, and
+          // each stores eight columns of one run
+          uint16_t b[2][4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) store_val<DT>(b[h], v, y[h][v]);
+          uint32_t w[2][2];
+          __builtin_memcpy(w, b, 16);
+          const auto x0 = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+          const auto x1 = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+          const int n = first - 4 * lk + 8 * (g + lk);
+          if (in && n < a.N) *reinterpret_cast<uint4*>((uint16_t*)a.Y + row + n) = make_uint4(x0[0], x1[0], x0[1], x1[1]);
+        } else if (in) {
+          store_run<DT>(a.Y, row, first + 8 * g, a.N, a.vec_out, y[0]);
+          store_run<DT>(a.Y, row, first + 8 * g + 8, a.N, a.vec_out, y[1]);
+        }
+      }
     }
   }
 
@@ -520,7 +561,7 @@ struct TileKernel {
     int id;
     if (!order.next(whole, id)) return;
     Job now = job(whole, id);
-    int buf = 0;
+    int buf = 0, half = 0;
     if (a.rows) {
       if (threadIdx.x < TM) sh.rows[0][threadIdx.x] = a.rows[min(now.m0 + (int)threadIdx.x, now.mend - 1)];
       __syncthreads();
@@ -541,6 +582,7 @@ struct TileKernel {
       if (a.rows)  // rows 32 wave .. 32 wave + 31, two words each
         load_lds4((const int*)(a.rows + min(after.m0 + 32 * wave + (lane >> 1), after.mend - 1)) + (lane & 1),
                   rows0 + (unsigned)(buf1 * TM + 32 * wave) * 8u);
+      load_scales(now, buf, half);
       first_fragments();
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -555,7 +597,8 @@ struct TileKernel {
       else if (rows > 32) loop<2>(after, buf1);
       else if (rows > 0) loop<1>(after, buf1);
       else loop<0>(after, buf1);
-      results(now, buf);
+      results(now, half);
+      half ^= 1;
       if (!more) break;
       now = after;
       buf = buf1;
@@ -999,6 +1042,7 @@ int int8_dispatch(Int8Args a, int dtype, int swiglu, int8_t* ws, hipStream_t st)
   // runs of four results leave in one store where rows of Y allow it
   const int run = dtype == DT_F32 ? 16 : 8;
   a.vec_out = a.N % 4 == 0 && ((uintptr_t)a.Y % run) == 0 && a.ldy % 4 == 0;
+  if (a.vec_out && a.N % 8 == 0 && ((uintptr_t)a.Y % 16) == 0 && a.ldy % 8 == 0) a.vec_out = 2;
   if (dtype == DT_F32) return swiglu ? int8_launch<DT_F32, true>(a, st) : int8_launch<DT_F32, false>(a, st);
   if (dtype == DT_BF16) return swiglu ? int8_launch<DT_BF16, true>(a, st) : int8_launch<DT_BF16, false>(a, st);
   return swiglu ? int8_launch<DT_F16, true>(a, st) : int8_launch<DT_F16, false>(a, st);
