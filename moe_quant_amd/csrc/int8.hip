@@ -21,6 +21,16 @@ __device__ __forceinline__ float load_val(const void* p, long i) {
   if (DT == DT_BF16) return bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(p)[i]);
   return (float)reinterpret_cast<const _Float16*>(p)[i];
 }
+// two results in 16 bits each, rounded to nearest, ties to even (one instruction for bf16 on this chip)
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  typedef float floatx2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  const floatx2 v = {a, b};
+  if (DT == DT_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
+}
 template <int DT>
 __device__ __forceinline__ void store_val(void* p, long i, float v) {
   if (DT == DT_F32) reinterpret_cast<float*>(p)[i] = v;
@@ -198,12 +208,7 @@ __device__ __forceinline__ void store_run(void* Y, long row, int n, int N, int v
     if (DT == DT_F32) {
       *reinterpret_cast<float4*>((float*)Y + row + n) = float4{y[0], y[1], y[2], y[3]};
     } else {
-      uint16_t h[4];
-#pragma unroll
-      for (int v = 0; v < 4; ++v) store_val<DT>(h, v, y[v]);
-      uint2 w;
-      __builtin_memcpy(&w, h, 8);
-      *reinterpret_cast<uint2*>((uint16_t*)Y + row + n) = w;
+      *reinterpret_cast<uint2*>((uint16_t*)Y + row + n) = make_uint2(pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3]));
     }
   } else {
 #pragma unroll
@@ -502,15 +507,8 @@ struct TileKernel {
         if (DT != DT_F32 && a.vec_out == 2) {
           // lanes l and l + 32 hold columns 8 g .. + 3 and + 4 .. + 7 of one row, and the same of the next run: they swap, and
           // each stores eight columns of one run
-          uint16_t b[2][4];
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int v = 0; v < 4; ++v) store_val<DT>(b[h], v, y[h][v]);
-          uint32_t w[2][2];
-          __builtin_memcpy(w, b, 16);
-          const auto x0 = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
-          const auto x1 = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+          const auto x0 = __builtin_amdgcn_permlane32_swap(pack2<DT>(y[0][0], y[0][1]), pack2<DT>(y[1][0], y[1][1]), false, false);
+          const auto x1 = __builtin_amdgcn_permlane32_swap(pack2<DT>(y[0][2], y[0][3]), pack2<DT>(y[1][2], y[1][3]), false, false);
           const int n = first - 4 * lk + 8 * (g + lk);
           if (in && n < a.N) *reinterpret_cast<uint4*>((uint16_t*)a.Y + row + n) = make_uint4(x0[0], x1[0], x0[1], x1[1]);
         } else if (in) {
