@@ -230,19 +230,20 @@ __device__ __forceinline__ intx4 short_row(const int8_t* row, int k, int K, bool
 }
 
 // Tiles of 256 x 256 for rows of at least 16 bytes that start at multiples of 4.  One workgroup per CU, eight wavefronts of
-// 128 x 64, takes one tile after the other; four stages of 64 bytes of every row in shared memory (128 KB), filled by
-// direct 16-byte loads.
-//   Layout of a stage: 256 token rows, then 256 weight rows, 64 bytes each; the 16-byte chunk c of row r lies at position
-//   c ^ (r / 4 % 4), so that 16 lanes reading chunk c of 16 rows touch every bank once.
-//   Pipeline: while the matrix instructions of one half of a stage run, the fragments of the other half are read; the loads
-//   of stage t + 4 are issued into the slot of stage t once every wavefront has read its last fragment (one barrier a
-//   stage, waits for exactly the loads that must have landed).  The stages of the next tile follow those of this one
-//   without a gap, so its first loads are in flight while this tile's results are written.
+// 128 x 64, takes one tile after the other; two stages of 128 bytes of every row in shared memory (128 KB), filled by
+// direct 16-byte loads, eight lanes to a row: whole 128-byte lines (64 bytes of every row at a time halve what memory gives:
+// the weights of partly filled tiles came in at 1.8 TB/s).
+//   Layout of a stage: 256 token rows, then 256 weight rows, 128 bytes each; the 16-byte chunk c of row r lies at position
+//   c ^ (r / 2 % 8), so that 16 lanes reading chunk c of 16 rows touch every bank once.
+//   Pipeline: a stage is four steps of 32 bytes; while the matrix instructions of one run, the fragments of the next are
+//   read.  Once every wavefront has read the last step's (one barrier a stage), the loads of the stage after the next are
+//   issued into the slot.  The stages of the next tile follow those of this one without a gap, so its first loads are in
+//   flight while this tile's results are written.
 //   The end of a row: a chunk that reaches beyond K is loaded from the last 16 bytes of the row instead (never outside it),
 //   and the tokens' fragments drop the bytes that belong to earlier chunks, or all of them.
 //   A wavefront computes only the 32-row blocks (NB of its four) that hold any rows.
-constexpr int TM = 256, TN = 256, TK = 64, NST = 4, STAGE = (TM + TN) * TK;
-constexpr int MIN_STAGES = 7;  // what the hand-over to the next tile needs; beyond K everything counts as zero
+constexpr int TM = 256, TN = 256, TK = 128, NST = 2, STAGE = (TM + TN) * TK;
+constexpr int MIN_STAGES = 3;  // what the hand-over to the next tile needs; beyond K everything counts as zero
 constexpr int MAX_GROUPS = 1024;
 struct TileShared {
   int8_t stage[NST][STAGE];
@@ -288,12 +289,13 @@ struct TileKernel {
   TileShared& sh;
   const int lane, wave, wm, wn, lr, lk;
   const int nk;         // stages of a tile
-  const int chunk;      // this lane's chunk of a stage's 64 bytes in direct loads
+  const int chunk;      // this lane's chunk of a stage's 128 bytes in direct loads of even number (of odd number: chunk ^ 4)
   const unsigned lds0;  // LDS address of the stages
   const unsigned rows0, scale0;
   intx16 acc[4][2];
-  intx4 fa0[4], fb0[2];
-  const int8_t *src[4], *next[4];
+  intx4 fa[2][4], fb[2][2];
+  int src[8], next[8];  // rows of this wavefront's direct loads: four of the tokens, four of the weights
+  const int8_t *from_a, *from_b, *next_b;
   int slot;
 
   __device__ __forceinline__ static unsigned lds_of(const void* p) {
@@ -302,7 +304,7 @@ struct TileKernel {
   __device__ __forceinline__ TileKernel(const Int8Args& args, TileShared& s)
       : a(args), sh(s), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), wm(wave >> 2),
         wn(wave & 3), lr(lane & 31), lk(lane >> 5), nk(max((args.K + TK - 1) / TK, MIN_STAGES)),
-        chunk((lane & 3) ^ (lane >> 4)), lds0(lds_of(&s.stage[0][0])), rows0(lds_of(&s.rows[0][0])), scale0(lds_of(&s.scale[0][0][0])),
+        chunk((lane & 7) ^ (lane >> 4)), lds0(lds_of(&s.stage[0][0])), rows0(lds_of(&s.rows[0][0])), scale0(lds_of(&s.scale[0][0][0])),
         slot(0) {}
 
   // Experts' ranges (clamped to [0, M]; a plain product is one expert's) and the whole and partly filled row tiles before
@@ -369,95 +371,83 @@ struct TileKernel {
     return j;
   }
 
-  // Where this wavefront's direct loads of a tile start: rows 32 wave + 16 q + lane / 4 of the tokens (q = 0, 1) and of the
-  // weights (q = 2, 3)
-  __device__ __forceinline__ void sources(const Job& j, int buf, const int8_t** p) const {
-    const int8_t* B = a.B + (long)j.e * a.strideB;
+  // The rows of this wavefront's direct loads (eight rows each): tokens' rows 32 wave + 8 q + lane / 8, and the weights'.
+  // Rows beyond a tile's are loaded as its last one, rows that are none as the first: their results are dropped or scaled by
+  // 0.
+  __device__ __forceinline__ void sources(const Job& j, int buf, int* rows, const int8_t** b) const {
+    *b = a.B + (long)j.e * a.strideB;
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int r = 32 * wave + 16 * q + (lane >> 2);
+    for (int q = 0; q < 4; ++q) {
+      const int r = 32 * wave + 8 * q + (lane >> 3);
       // SwiGLU: rows 0..31 of every 64 are gate rows, 32..63 the up rows of the same columns
       int col = SWIGLU ? j.n0 + (r >> 6) * 32 + (r & 31) : j.n0 + r;
       if (col >= a.N) col = j.n0;
-      p[2 + q] = B + (long)(SWIGLU && (r & 32) ? a.N + col : col) * a.ldb + 16 * chunk;
+      rows[4 + q] = SWIGLU && (r & 32) ? a.N + col : col;
       const long from = a.rows ? sh.rows[buf][r] : min(j.m0 + r, j.mend - 1);
-      p[q] = from >= 0 && from < a.src_rows ? a.A + from * a.lda + 16 * chunk : p[2 + q];
+      rows[q] = from >= 0 && from < a.src_rows ? (int)from : 0;
     }
   }
 
-  // stage s of this tile (of the next one, counted on, from nk on), load q
+  // all of stage s of this tile (of the next one, counted on, from nk on), load q
   __device__ __forceinline__ void issue(int s, int at_slot, int q) {
     const bool over = s >= nk;
-    const int k = TK * (over ? s - nk : s) + 16 * chunk;
-    const int off = min(k, a.K - 16) - 16 * chunk;
-    load_lds16((over ? next[q] : src[q]) + off,
-               lds0 + (unsigned)(at_slot * STAGE + (q >> 1) * TM * TK + wave * 2048 + (q & 1) * 1024));
+    const int k = TK * (over ? s - nk : s) + 16 * (q & 1 ? chunk ^ 4 : chunk);
+    const int off = min(k, a.K - 16);
+    const unsigned ld = (unsigned)(q < 4 ? a.lda : a.ldb);
+    const int8_t* base = q < 4 ? from_a : (over ? next_b : from_b);
+    load_lds16(base + (unsigned long)(unsigned)(over ? next[q] : src[q]) * ld + off,
+               lds0 + (unsigned)(at_slot * STAGE + (q >> 2) * TM * TK + wave * 4096 + (q & 3) * 1024));
   }
 
-  __device__ __forceinline__ void first_fragments() {
-    const int8_t* stg = sh.stage[slot];
-    const int at0 = 16 * (lk ^ ((lr >> 2) & 3));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) fa0[i] = *reinterpret_cast<const intx4*>(stg + (wm * 128 + i * 32 + lr) * TK + at0);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) fb0[j] = *reinterpret_cast<const intx4*>(stg + TM * TK + (wn * 64 + j * 32 + lr) * TK + at0);
+  // fragments of step `ks` of the stage in `at_slot`
+  template <int NB>
+  __device__ __forceinline__ void fragment(int at_slot, int ks, int c, intx4* ta, intx4* tb) const {
+    const int8_t* stg = sh.stage[at_slot];
+    const int at = 16 * ((2 * ks + lk) ^ ((lr >> 1) & 7));
+    if (c < NB) ta[c] = *reinterpret_cast<const intx4*>(stg + (wm * 128 + c * 32 + lr) * TK + at);
+    else tb[c - NB] = *reinterpret_cast<const intx4*>(stg + TM * TK + (wn * 64 + (c - NB) * 32 + lr) * TK + at);
   }
 
   // all stages of a tile; `after` is the next tile
   template <int NB>
   __device__ __forceinline__ void loop(const Job& after, int after_buf) {
-    constexpr int NJ = NB ? 2 : 0;  // a wavefront without rows only loads
-    const int pos = lk ^ ((lr >> 2) & 3);
-    const int a_off = (wm * 128 + lr) * TK, b_off = TM * TK + (wn * 64 + lr) * TK;
-    const int at0 = 16 * pos, at1 = 16 * (pos ^ 2);  // chunks lk and 2 + lk
-    intx4 fa1[4], fb1[2];
-    constexpr int MF = NB ? 2 * NB : 1, ACTS = NB + NJ + 2;  // matrix instructions of half a stage; reads and loads among them
+    constexpr int NR = NB ? NB + 2 : 0;   // fragments of a step; a wavefront without rows only loads
+    constexpr int MF = NB ? 2 * NB : 1;   // matrix instructions of a step
 #pragma unroll 1
     for (int kt = 0; kt < nk; ++kt) {
-      const int8_t* stg = sh.stage[slot];
-      const int before = (slot + NST - 1) % NST, here = slot;
-      slot = (slot + 1) % NST;
-      const int8_t* nxt = sh.stage[slot];
-      if (kt == 3) sources(after, after_buf, next);  // (the row numbers were loaded before kt = 0: landed by now)
+      if (kt == 1) sources(after, after_buf, next, &next_b);  // (the row numbers were loaded before kt = 0: landed by now)
+      const int here = slot, there = slot ^ 1;
       const bool ragged = TK * (kt + 1) > a.K;
-      if (ragged) {
-        const int d = max(0, TK * kt + 16 * lk - (a.K - 16));
 #pragma unroll
-        for (int i = 0; i < NB; ++i) fa0[i] = keep_from(fa0[i], d);
+      for (int ks = 0; ks < 4; ++ks) {
+        if (ks == 3) {
+          asm volatile("" ::: "memory");
+          __builtin_amdgcn_s_waitcnt(0x0070);  // the next stage landed, this one's last fragments are read
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+        }
+        if (ragged) {
+          const int d = max(0, TK * kt + 32 * ks + 16 * lk - (a.K - 16));
+#pragma unroll
+          for (int i = 0; i < NB; ++i) fa[ks & 1][i] = keep_from(fa[ks & 1][i], d);
+        }
+        constexpr int ACTS3 = NR + 8;
+#pragma unroll
+        for (int m = 0; m < MF; ++m) {
+          if (NB)
+            acc[m >> 1][m & 1] =
+                __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[ks & 1][m & 1], fa[ks & 1][m >> 1], acc[m >> 1][m & 1], 0, 0, 0);
+          const int acts = ks == 3 ? ACTS3 : NR;
+#pragma unroll
+          for (int c = 0; c < ACTS3; ++c)
+            if (c < acts && c * MF / acts == m) {
+              if (c < NR) fragment<NB>(ks == 3 ? there : here, (ks + 1) & 3, c, fa[(ks + 1) & 1], fb[(ks + 1) & 1]);
+              else issue(kt + NST, here, c - NR);
+            }
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
-#pragma unroll
-      for (int m = 0; m < MF; ++m) {
-        if (NB) acc[m >> 1][m & 1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb0[m & 1], fa0[m >> 1], acc[m >> 1][m & 1], 0, 0, 0);
-#pragma unroll
-        for (int c = 0; c < ACTS; ++c)
-          if (c * MF / ACTS == m) {
-            if (c < NB) fa1[c] = *reinterpret_cast<const intx4*>(stg + a_off + at1 + c * 32 * TK);
-            else if (c < NB + NJ) fb1[c - NB] = *reinterpret_cast<const intx4*>(stg + b_off + at1 + (c - NB) * 32 * TK);
-            else issue(kt + NST - 1, before, 2 + c - NB - NJ);
-          }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_s_waitcnt(0x0070 | 8);  // the next stage landed: at most the 8 loads of the two after it in flight
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      if (ragged) {
-        const int d = max(0, TK * kt + 32 + 16 * lk - (a.K - 16));
-#pragma unroll
-        for (int i = 0; i < NB; ++i) fa1[i] = keep_from(fa1[i], d);
-      }
-#pragma unroll
-      for (int m = 0; m < MF; ++m) {
-        if (NB) acc[m >> 1][m & 1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb1[m & 1], fa1[m >> 1], acc[m >> 1][m & 1], 0, 0, 0);
-#pragma unroll
-        for (int c = 0; c < ACTS; ++c)
-          if (c * MF / ACTS == m) {
-            if (c < NB) fa0[c] = *reinterpret_cast<const intx4*>(nxt + a_off + at0 + c * 32 * TK);
-            else if (c < NB + NJ) fb0[c - NB] = *reinterpret_cast<const intx4*>(nxt + b_off + at0 + (c - NB) * 32 * TK);
-            else issue(kt + NST, here, c - NB - NJ);
-          }
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      slot = there;
     }
   }
 
@@ -564,13 +554,14 @@ struct TileKernel {
       if (threadIdx.x < TM) sh.rows[0][threadIdx.x] = a.rows[min(now.m0 + (int)threadIdx.x, now.mend - 1)];
       __syncthreads();
     }
-    sources(now, 0, src);
+    from_a = a.src_rows > 0 ? a.A : a.B;  // (no rows at all: anything that can be read)
+    sources(now, 0, src, &from_b);
 #pragma unroll
     for (int s = 0; s < NST; ++s)
 #pragma unroll
-      for (int q = 0; q < (s < NST - 1 ? 4 : 2); ++q) issue(s, s, q);
+      for (int q = 0; q < 8; ++q) issue(s, s, q);
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0070 | 10);  // stage 0 landed: at most the 10 loads of stages 1, 2, 3 in flight
+    __builtin_amdgcn_s_waitcnt(0x0070 | 8);  // stage 0 landed
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     for (;;) {
@@ -581,7 +572,8 @@ struct TileKernel {
         load_lds4((const int*)(a.rows + min(after.m0 + 32 * wave + (lane >> 1), after.mend - 1)) + (lane & 1),
                   rows0 + (unsigned)(buf1 * TM + 32 * wave) * 8u);
       load_scales(now, buf, half);
-      first_fragments();
+#pragma unroll
+      for (int c = 0; c < 6; ++c) fragment<4>(slot, 0, c, fa[0], fb[0]);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -601,7 +593,8 @@ struct TileKernel {
       now = after;
       buf = buf1;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) src[q] = next[q];
+      for (int q = 0; q < 8; ++q) src[q] = next[q];
+      from_b = next_b;
     }
     __builtin_amdgcn_s_waitcnt(0x0070);
   }
@@ -967,7 +960,7 @@ int vector_launch(const Int8Args& a, hipStream_t st) {
   return mq_check_launch();
 }
 
-bool rows_of_words(const int8_t* p, long ld) { return ((uintptr_t)p & 3) == 0 && ld % 4 == 0; }
+bool rows_of_words(const int8_t* p, long ld) { return ((uintptr_t)p & 3) == 0 && ld % 4 == 0 && ld < 0x7fffffff; }
 
 // the vector kernel takes one or two rows whose codes fit its shared memory
 bool for_vector(int M, int K) { return M <= VT && K >= 16 && vector_smem(K) <= 160 * 1024; }
