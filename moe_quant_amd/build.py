@@ -11,7 +11,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_PATH = os.path.join(HERE, "libmoequant_hip.so")
 SOURCES = ["gemm_f32.hip", "syrk_bf16.hip", "factor.hip", "gptq_loop.hip", "prep_pack.hip", "hygiene.hip", "routing.hip", "route_f32.hip",
-           "route_bf16.hip", "route_f16.hip", "int8.hip"]
+           "route_bf16.hip", "route_f16.hip", "int8.hip", "int8_f32.hip", "int8_bf16.hip", "int8_f16.hip"]
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",
     "-O3",
