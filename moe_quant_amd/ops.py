@@ -24,7 +24,8 @@ def _dt(dtype: Optional[torch.dtype]) -> int:
 
 
 def _stream(t: Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    # the handle of torch.cuda.current_stream(t.device), without building a Stream object for it (2 us of a small call's 11)
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def _dev(*ts: Optional[Tensor]) -> None:
