@@ -117,7 +117,7 @@ __global__ __launch_bounds__(256) void align_rows_kernel(const int8_t* __restric
 size_t padded(int K) { return ((size_t)K + 15) / 16 * 16; }
 // K no multiple of 4: contiguous rows start anywhere; large products copy them first (30 us for 8192 x 7781 weights against
 // the millisecond that such rows cost a product of 4096 tokens)
-bool aligns_rows(int M, int N, int K, int swiglu) { return K % 4 != 0 && K >= 16 && enough_tiles(M, N, swiglu, 128, 96); }
+bool aligns_rows(int M, int N, int K, int swiglu) { return K % 4 != 0 && K >= 16 && small_tiles(M, N, swiglu); }
 
 int int8_dispatch(Int8Args a, int dtype, int swiglu, int8_t* ws, hipStream_t st) {
   if (ws && aligns_rows(a.M, a.N, a.K, swiglu)) {

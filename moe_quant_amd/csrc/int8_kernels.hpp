@@ -562,13 +562,20 @@ int tile_launch(const Int8Args& a, hipStream_t st) {
   return mq_check_launch();
 }
 
-// Few rows or few tiles: a workgroup computes 16 R x 16 C results, its eight wavefronts an eighth of K each, with fragments
-// straight from memory (16 rows x 64 bytes an instruction, UN of them in flight) -- every weight byte of the tile is used by
-// one wavefront only, so shared memory would add nothing but latency.  The eight sums meet in shared memory.  Grouped: a
-// workgroup belongs to an expert and walks over its rows in steps of 16 R.  Any alignment, any K.
-template <int DT, bool SWIGLU, int R, int C, int UN>
-__global__ __launch_bounds__(512) void int8_thin_kernel(Int8Args a, int gx) {
-  __shared__ intx4 part[8][R * C][64];
+// Few rows or few tiles: a workgroup computes 16 R x 16 C results, its eight wavefronts an eighth of K each; the eight sums meet
+// in shared memory.  Grouped: a workgroup belongs to an expert and walks over its rows in steps of 16 R.
+//   D > 0, for rows of at least 16 bytes that start at multiples of 4: a wavefront keeps D - 1 steps of 64 bytes of its rows on
+//   their way into shared memory of its own by direct loads, four lanes to a row.  (Fragments want lane l to hold row l % 16:
+//   loaded like that, an instruction touches every row four times and the address unit takes 64 cycles for it.)  Chunk c of
+//   row r lies at position c ^ (r / 4 % 4): 16 lanes reading chunk c of 16 rows touch every bank once.
+//   D = 0: fragments straight from memory, UN steps at a time; any alignment, any K.
+constexpr int vmcnt_is(int n) { return 0x0070 | (n & 15) | (n >> 4) << 14; }  // ... and lgkmcnt(0)
+
+template <int DT, bool SWIGLU, int R, int C, int UN, int D>
+__global__ __launch_bounds__(512) void int8_thin_kernel(Int8Args a, int gx, int by_row) {
+  extern __shared__ __attribute__((aligned(1024))) int8_t smem[];
+  typedef intx4 Sums[R * C][64];
+  Sums* part = reinterpret_cast<Sums*>(smem);  // of every wavefront (where its steps were)
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, lq = lane >> 4;
@@ -577,18 +584,26 @@ __global__ __launch_bounds__(512) void int8_thin_kernel(Int8Args a, int gx) {
   int e = 0, mbeg = by * 16 * R, mend = min(mbeg + 16 * R, a.M);
   if (a.offsets) {
     e = by;
+    if (by_row) {  // the expert of row `by`: as many as end before it or with it come first
+      e = 0;
+#pragma unroll 4
+      for (int e0 = 0; e0 < a.E; e0 += 64) e += __popcll(__ballot(e0 + lane < a.E && a.offsets[min(e0 + lane, a.E - 1) + 1] <= by));
+      if (e >= a.E) return;
+    }
     mbeg = (int)min(max(a.offsets[e], 0l), (long)a.M);
     mend = (int)min(max(a.offsets[e + 1], (long)mbeg), (long)a.M);
+    if (by_row && mbeg != by) return;  // its first row's workgroup does them all
   }
   const int8_t* B = a.B + (long)e * a.strideB;
   const float* sb = a.sb + (long)e * (SWIGLU ? 2 * a.N : a.N);
   const int steps = (a.K + 63) >> 6, per = (steps + 7) >> 3;
   const int k0 = 64 * per * wave, k1 = min(a.K, k0 + 64 * per);
+  const int lrow = D ? lane >> 2 : l16;  // the row this lane loads of every 16
   const int8_t* brow[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     // SwiGLU: even blocks of 16 are gate rows, odd ones the up rows of the same columns
-    int col = SWIGLU ? n0 + 16 * (c >> 1) + l16 : n0 + 16 * c + l16;
+    int col = SWIGLU ? n0 + 16 * (c >> 1) + lrow : n0 + 16 * c + lrow;
     if (col >= a.N) col = n0;
     brow[c] = B + (long)(SWIGLU && (c & 1) ? a.N + col : col) * a.ldb;
   }
@@ -597,58 +612,106 @@ __global__ __launch_bounds__(512) void int8_thin_kernel(Int8Args a, int gx) {
     bool ain[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int m = m0 + 16 * r + l16;
+      const int m = m0 + 16 * r + lrow;
       long from = m;
       ain[r] = m < mend;
       if (ain[r] && a.rows) from = a.rows[m];
       ain[r] = ain[r] && from >= 0 && from < a.src_rows;
-      arow[r] = a.A + (ain[r] ? from : 0) * a.lda;
+      // (a row that is none is loaded from the weights: its results are dropped, or scaled by 0)
+      arow[r] = ain[r] ? a.A + from * a.lda : brow[0];
     }
     intx4 acc[R][C];
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int c = 0; c < C; ++c) acc[r][c] = intx4{0, 0, 0, 0};
-    if (a.K < 16 && wave == 0) {
-      intx4 ta[R], tb[C];
+    if (m0 != mbeg) __syncthreads();  // the sums of the rows before have been read
+    if (D > 0) {
+      const int mine = k1 > k0 ? (k1 - k0 + 63) >> 6 : 0;
+      const int chunk = (lane & 3) ^ lq;
+      int8_t* slots = smem + wave * (D ? D : 1) * (R + C) * 1024;
+      const unsigned lds0 = __builtin_amdgcn_readfirstlane(
+          (unsigned)(uintptr_t)(__attribute__((address_space(3))) int8_t*)slots);
+      // (steps past the last load it again into slots nobody reads: the waits keep their counts)
+      const auto issue = [&](int s, int slot) {
+        const int off = min(k0 + 64 * min(s, mine - 1) + 16 * chunk, a.K - 16);
 #pragma unroll
-      for (int c = 0; c < C; ++c) tb[c] = short_row(brow[c], 16 * lq, a.K, true);
+        for (int r = 0; r < R; ++r) load_lds16(arow[r] + off, lds0 + (unsigned)(slot * (R + C) + r) * 1024u);
 #pragma unroll
-      for (int r = 0; r < R; ++r) ta[r] = short_row(arow[r], 16 * lq, a.K, ain[r]);
+        for (int c = 0; c < C; ++c) load_lds16(brow[c] + off, lds0 + (unsigned)(slot * (R + C) + R + c) * 1024u);
+      };
+      if (mine > 0) {
 #pragma unroll
-      for (int r = 0; r < R; ++r)
+        for (int s = 0; s < D - 1; ++s) issue(s, s);
+        int slot = 0;
+        const int at = l16 * 64 + 16 * (lq ^ (l16 >> 2));
+#pragma unroll 1
+        for (int t = 0; t < mine; ++t) {
+          asm volatile("" ::: "memory");
+          __builtin_amdgcn_s_waitcnt(vmcnt_is((D > 1 ? D - 2 : 0) * (R + C)));  // step t landed; the last step's fragments are read
+          asm volatile("" ::: "memory");
+          const int8_t* here = slots + slot * (R + C) * 1024 + at;
+          intx4 fa[R], fb[C];
 #pragma unroll
-        for (int c = 0; c < C; ++c) acc[r][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(tb[c], ta[r], acc[r][c], 0, 0, 0);
-    }
-    for (int k = a.K < 16 ? k1 : k0; k < k1; k += 64 * UN) {
-      intx4 fa[UN][R], fb[UN][C];
+          for (int r = 0; r < R; ++r) fa[r] = *reinterpret_cast<const intx4*>(here + r * 1024);
 #pragma unroll
-      for (int u = 0; u < UN; ++u) {
-        // chunks beyond the end of a row: the weights' last 16 bytes once more, against zeros
-        const int kc = k + 64 * u + 16 * lq, at = min(kc, a.K - 16);
+          for (int c = 0; c < C; ++c) fb[c] = *reinterpret_cast<const intx4*>(here + (R + c) * 1024);
+          issue(t + D - 1, slot == 0 ? D - 1 : slot - 1);
+          slot = slot == D - 1 ? 0 : slot + 1;
+          const int kc = k0 + 64 * t;
+          if (kc + 64 > a.K) {
 #pragma unroll
-        for (int c = 0; c < C; ++c) __builtin_memcpy(&fb[u][c], brow[c] + at, 16);
+            for (int r = 0; r < R; ++r) fa[r] = keep_from(fa[r], max(0, kc + 16 * lq - (a.K - 16)));
+          }
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          fa[u][r] = intx4{0, 0, 0, 0};
-          if (ain[r] && kc < k1) __builtin_memcpy(&fa[u][r], arow[r] + at, 16);
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int c = 0; c < C; ++c) acc[r][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[c], fa[r], acc[r][c], 0, 0, 0);
         }
+        __builtin_amdgcn_s_waitcnt(0x0070);
       }
+      __syncthreads();  // the sums go where the steps were
+    } else {
+      if (a.K < 16 && wave == 0) {
+        intx4 ta[R], tb[C];
 #pragma unroll
-      for (int u = 0; u < UN; ++u) {
-        const int kc = k + 64 * u + 16 * lq;
-        if ((a.K & 15) && a.K > 16) {
+        for (int c = 0; c < C; ++c) tb[c] = short_row(brow[c], 16 * lq, a.K, true);
 #pragma unroll
-          for (int r = 0; r < R; ++r) fa[u][r] = keep_from(fa[u][r], kc - (a.K - 16));
-        }
+        for (int r = 0; r < R; ++r) ta[r] = short_row(arow[r], 16 * lq, a.K, ain[r]);
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
-          for (int c = 0; c < C; ++c)
-            acc[r][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[u][c], fa[u][r], acc[r][c], 0, 0, 0);
+          for (int c = 0; c < C; ++c) acc[r][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(tb[c], ta[r], acc[r][c], 0, 0, 0);
+      }
+      for (int k = a.K < 16 ? k1 : k0; k < k1; k += 64 * UN) {
+        intx4 fa[UN][R], fb[UN][C];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+          // chunks beyond the end of a row: the weights' last 16 bytes once more, against zeros
+          const int kc = k + 64 * u + 16 * lq, at = min(kc, a.K - 16);
+#pragma unroll
+          for (int c = 0; c < C; ++c) __builtin_memcpy(&fb[u][c], brow[c] + at, 16);
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            fa[u][r] = intx4{0, 0, 0, 0};
+            if (ain[r] && kc < k1) __builtin_memcpy(&fa[u][r], arow[r] + at, 16);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+          const int kc = k + 64 * u + 16 * lq;
+          if ((a.K & 15) && a.K > 16) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) fa[u][r] = keep_from(fa[u][r], kc - (a.K - 16));
+          }
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+              acc[r][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[u][c], fa[u][r], acc[r][c], 0, 0, 0);
+        }
       }
     }
-    if (m0 != mbeg) __syncthreads();  // the sums of the rows before have been read
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -684,12 +747,28 @@ __global__ __launch_bounds__(512) void int8_thin_kernel(Int8Args a, int gx) {
   }
 }
 
-template <int DT, bool SWIGLU, int R, int C, int UN>
+template <int DT, bool SWIGLU, int R, int C, int UN, int D>
 int thin_launch(const Int8Args& a, hipStream_t st) {
+  constexpr int SMEM = 8 * 1024 * (D * (R + C) > R * C ? D * (R + C) : R * C);
+  static_assert(SMEM <= 160 * 1024, "shared memory of a CU");
+  if (SMEM > 48 * 1024) {
+    static std::atomic<uint64_t> set{0};  // GPUs on which the kernel may take its shared memory
+    int dev = -1;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return MQ_ERR_LAUNCH;
+    if (!(set.load() >> dev & 1)) {
+      if (hipFuncSetAttribute((const void*)int8_thin_kernel<DT, SWIGLU, R, C, UN, D>,
+                              hipFuncAttributeMaxDynamicSharedMemorySize, SMEM) != hipSuccess)
+        return MQ_ERR_LAUNCH;
+      set.fetch_or(1ull << dev);
+    }
+  }
   const int outn = SWIGLU ? 8 * C : 16 * C, gx = (a.N + outn - 1) / outn;
-  const long grid = (long)gx * (a.offsets ? a.E : (a.M + 16 * R - 1) / (16 * R));
+  // fewer rows than experts: a workgroup a row (the others of its expert's leave at once) rather than one an expert, most
+  // of which would have no rows: 16384 that leave at once take 25 us
+  const int by_row = a.offsets && a.M < a.E;
+  const long grid = (long)gx * (a.offsets ? min(a.M, a.E) : (a.M + 16 * R - 1) / (16 * R));
   if (grid > 0x7fffffffL) return MQ_ERR_TOO_LARGE;
-  hipLaunchKernelGGL((int8_thin_kernel<DT, SWIGLU, R, C, UN>), dim3((unsigned)grid), dim3(512), 0, st, a, gx);
+  hipLaunchKernelGGL((int8_thin_kernel<DT, SWIGLU, R, C, UN, D>), dim3((unsigned)grid), dim3(512), SMEM, st, a, gx, by_row);
   return mq_check_launch();
 }
 
@@ -905,6 +984,7 @@ bool for_vector(int M, int K) { return M <= VT && K >= 16 && vector_smem(K) <= 1
 bool enough_tiles(int M, int N, int swiglu, int edge, int count) {
   return ((long)M + edge - 1) / edge * (((long)N * (swiglu ? 2 : 1) + edge - 1) / edge) >= count;
 }
+bool small_tiles(int M, int N, int swiglu) { return M > 32 && enough_tiles(M, N, swiglu, 128, 136); }
 // a grouped product's tiles of 256 x 256, at most
 template <bool SWIGLU>
 bool enough_jobs(const Int8Args& a) {
@@ -917,7 +997,8 @@ int int8_launch(const Int8Args& a, hipStream_t st) {
   if (a.offsets) {
     // A decode step: 110 + 71 us without shared memory against 139 + 70 with tiles at 32 rows over 64 experts of 7168 x 2048,
     // 201 + 125 against 205 + 125 at 128 rows; at 512 rows the tiles win, 296 + 195 against 388 + 217.
-    if (!tiles || a.M <= 4l * a.E) return thin_launch<DT, SWIGLU, 2, 2, 2>(a, st);
+    // (Staging the rows costs there: 130 + 78.)
+    if (!tiles || a.M <= 4l * a.E) return thin_launch<DT, SWIGLU, 2, 2, 2, 0>(a, st);
     // Few rows an expert: the weights' bytes decide, and two small workgroups a CU keep more of them in flight (5.8 against
     // 4.9 TB/s at 32 rows for each of 128 experts of 7168 x 2048).  Many rows: large tiles read both operands less often
     // (1830 against 1480 TOP/s at 256 rows), if there are enough of them to go round several times.
@@ -927,19 +1008,23 @@ int int8_launch(const Int8Args& a, hipStream_t st) {
   if (for_vector(a.M, a.K)) return vector_launch<DT, SWIGLU, -1>(a, st);
   // 76 us at 4096 x 4096 x 4096 (256 large tiles) against 103 with small ones; 57 against 48 at 2048 x 4096 x 4096 (128)
   if (tiles && enough_tiles(a.M, a.N, SWIGLU, 256, 192)) return tile_launch<DT, SWIGLU, 256>(a, st);
-  // 33 us at 512 x 4096 x 4096 (128 small tiles) against 38 without shared memory, 60 against 72 at 64 x 18432 x 7168; 17
-  // against 12 at 512 x 2048 x 2048 (64 tiles), 57 against 42 at 16 x 18432 x 7168 (tiles an eighth full)
-  if (tiles && a.M > 32 && enough_tiles(a.M, a.N, SWIGLU, 128, 96)) return tile_launch<DT, SWIGLU, 128>(a, st);
-  // the largest block of results that still gives 192 workgroups
+  // 62 us at 128 x 18432 x 7168 (144 small tiles) against 80 without tiles; 34 against 30 at 512 x 4096 x 4096 (128)
+  if (tiles && small_tiles(a.M, a.N, SWIGLU)) return tile_launch<DT, SWIGLU, 128>(a, st);
+  // the largest block of results that still gives 192 workgroups (and is half full, at least)
   const auto groups = [&](int R, int C) {
     const int outn = SWIGLU ? 8 * C : 16 * C;
-    return (long)((a.M + 16 * R - 1) / (16 * R)) * ((a.N + outn - 1) / outn);
+    return a.M > 8 * R || R == 1 ? (long)((a.M + 16 * R - 1) / (16 * R)) * ((a.N + outn - 1) / outn) : 0l;
   };
-  if (groups(4, 4) >= 192) return thin_launch<DT, SWIGLU, 4, 4, 1>(a, st);  // 12 us at 512 x 2048 x 2048, (2, 4) 17, (2, 2) 19
-  if (groups(2, 4) >= 192) return thin_launch<DT, SWIGLU, 2, 4, 4>(a, st);  // 9.3 us at 256 x 2048 x 2048, (4, 4) 12, (2, 2) 11
-  if (groups(2, 2) >= 192) return thin_launch<DT, SWIGLU, 2, 2, 2>(a, st);  // 16 us at 333 x 576 x 7168, (4, 4) 30, (1, 1) 23
-  if (groups(1, 2) >= 192 || SWIGLU) return thin_launch<DT, SWIGLU, 1, 2, 2>(a, st);  // 42 us at 16 x 18432 x 7168, (1, 1) 45
-  return thin_launch<DT, SWIGLU, 1, SWIGLU ? 2 : 1, 4>(a, st);  // 8.6 us at 8 x 2048 x 7168, (1, 2) 11
+  if (!tiles) {  // 16 us at 333 x 576 x 7168 against 12 for aligned rows
+    if (groups(4, 4) >= 192) return thin_launch<DT, SWIGLU, 4, 4, 1, 0>(a, st);
+    if (groups(2, 2) >= 192) return thin_launch<DT, SWIGLU, 2, 2, 2, 0>(a, st);
+    return thin_launch<DT, SWIGLU, 1, 2, 2, 0>(a, st);
+  }
+  if (groups(4, 4) >= 192) return thin_launch<DT, SWIGLU, 4, 4, 1, 2>(a, st);  // 11 us at 512 x 2048 x 2048, (2, 4) 14, (2, 2) 15
+  if (groups(2, 4) >= 192) return thin_launch<DT, SWIGLU, 2, 4, 1, 2>(a, st);  // 23 us at 64 x 7168 x 7168, (4, 4) 32, (2, 2) 27
+  if (groups(2, 2) >= 192) return thin_launch<DT, SWIGLU, 2, 2, 1, 2>(a, st);  // 12 us at 333 x 576 x 7168, (2, 4) 17, (1, 1) 16
+  if (groups(1, 2) >= 192 || SWIGLU) return thin_launch<DT, SWIGLU, 1, 2, 1, 3>(a, st);  // 4.8 us at 64 x 2048 x 2048, (1, 1) 5.8
+  return thin_launch<DT, SWIGLU, 1, SWIGLU ? 2 : 1, 1, 4>(a, st);  // 6.5 us at 8 x 2048 x 7168, (1, 2) 8.7
 }
 
 }  // namespace
