@@ -14,6 +14,9 @@ constexpr int ROUTE_MAX_E = 1024;
 // ---- sort by expert -----------------------------------------------------------------------------------
 // Stable counting sort of n = T * top_k choices into E + 1 bins (bin E: ids outside [0, E)).  A workgroup owns a run of
 // SORT_CHUNK choices; `count` holds, bin-major, the number of choices of every (bin, workgroup).
+// Measured: 144 us for 16.8 million choices over 256 experts (35 counting, 7 summing, 102 placing: 3.3 TB/s of its bytes), 5 us
+// for 488 in one workgroup.  Tried: chunks of 4096 and 16384 (108 and 120 us placing); putting a workgroup's choices in order
+// in shared memory first, so that rows leaves in runs (121).
 constexpr int SORT_CHUNK = 8192;
 constexpr int SORT_WAVES = 8;
 constexpr int SORT_MAX_E = 1024;
@@ -161,7 +164,8 @@ __global__ __launch_bounds__(512) void sort_scatter_kernel(const long* __restric
 
 // ---- combine --------------------------------------------------------------------------------------------
 // One workgroup per (token, 2048 columns); the sum runs in the order of the token's choices, in 32 bits, and is rounded
-// once.  Slots outside [0, S) add nothing.
+// once.  Slots outside [0, S) add nothing.  Bound by memory: 220 us for 8192 tokens of eight experts, 7168 bf16 columns (4.8
+// TB/s).
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void combine_kernel(const void* __restrict__ Y, long ldy, int S, int C,
                                                       const int* __restrict__ slots, const float* __restrict__ weights, int k,
