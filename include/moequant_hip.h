@@ -318,7 +318,7 @@ int mq_swiglu_packed(const void* G, long ldg, const void* U, long ldu, int n, in
  * first, ties (of runs too) to the lowest index; the choice is what 64-bit scores give.  weight = s, divided by the sum
  * over the chosen (+ 1e-20) if renormalize, times scale.
  *   logits : T x E (ldl) of type dtype; bias : E fp32, nullable; weights : T x top_k fp32; ids : T x top_k int64.
- *   score : 0 softmax, 1 sigmoid.  E <= 1024, top_k <= 64, n_group <= 64, top_k <= topk_group * E / n_group.
+ *   T <= 2^25 (MQ_ERR_TOO_LARGE beyond).  score : 0 softmax, 1 sigmoid.  E <= 1024, top_k <= 64, n_group <= 64, top_k <= topk_group * E / n_group.
  *   A NaN logit or bias counts as -inf; a row of -inf scores 0 (weights 0, ids still valid and distinct). */
 int mq_route_experts(const void* logits, int dtype, long ldl, int T, int E, int top_k, int score, const float* bias,
                      int n_group, int topk_group, int group_top, int renormalize, float scale, float* weights, long* ids,
@@ -334,11 +334,12 @@ int mq_sort_by_expert(const long* ids, int T, int top_k, int E, long* rows, long
                       size_t workspace_bytes, void* stream);
 
 /* out[t, :] = sum_j weights[t, j] * Y[slots[t, j], :], summed in fp32 in the order of j and rounded once; slots outside
- * [0, S) add nothing.  Y : S x C (ldy), out : T x C (ldo), both of type dtype; out must not overlap Y. */
+ * [0, S) add nothing.  Y : S x C (ldy), out : T x C (ldo), both of type dtype; out must not overlap Y.  C <= 2^26. */
 int mq_combine_experts(const void* Y, int dtype, long ldy, int S, int C, const int* slots, const float* weights, int T, int k,
                        void* out, long ldo, void* stream);
 
 /* ---- (6) products on 8-bit integers ----------------------------------------------------------------------------
+ * Row and column counts stay below 2^31 - 4096 (weights' rows below half of that).
  * Runs what GPTQ with 8 bits and one group per row yields (src/gptq.py:156-218: codes minus zero point, one scale per
  * output channel).
  * Tokens: scale[r] = max|X[r, :]| / 127 and Q[r, c] = 127 X[r, c] / max|X[r, :]| rounded to the nearest whole number, ties
@@ -367,7 +368,7 @@ int mq_linear_int8(const void* X, int dtype, long ldx, const int8_t* B, long ldb
 /* The same with weights per run of rows: rows offsets[e] .. offsets[e + 1) - 1 of Y (device array of E + 1 values, clamped
  * to [0, S]) are products with B + e * strideB, b_scale + e * N (swiglu: e * 2 N).  Row m of Y takes row rows[m] of A and
  * a_scale (rows : S int64 on the device; a value outside [0, src_rows) stands for a row of zeros) or, rows == NULL, row
- * m.  Rows of Y outside every range are left as they are.  E <= 1024. */
+ * m.  Rows of Y outside every range are left as they are.  E <= 1024.  src_rows == 0: A and a_scale may be NULL. */
 int mq_matmul_int8_grouped(const int8_t* A, long lda, const float* a_scale, int src_rows, const long* rows, int S,
                            const int8_t* B, long ldb, long strideB, const float* b_scale, int E, const long* offsets, void* Y,
                            long ldy, int out_dtype, int N, int K, int swiglu, void* stream);

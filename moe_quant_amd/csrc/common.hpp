@@ -18,6 +18,15 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef short bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8n __attribute__((ext_vector_type(8)));
 
+// largest row or column count of the routing and 8-bit entry points: rounding one up to a tile stays inside 32 bits
+#define MQ_MAX_COUNT (0x7fffffff - 4096)
+
+// `groups` workgroups in two dimensions (one takes fewer than 2^32 threads); the kernel's own: blockIdx.y * gridDim.x + blockIdx.x
+static inline dim3 mq_wide_grid(long groups, unsigned z = 1) {
+  const long x = groups < 65536 ? groups : 65536;
+  return dim3((unsigned)x, (unsigned)((groups + x - 1) / x), z);
+}
+
 static inline int mq_check_launch() { return hipGetLastError() == hipSuccess ? MQ_OK : MQ_ERR_LAUNCH; }
 
 __device__ __forceinline__ float bf16_bits_to_f32(uint16_t b) { return __uint_as_float(((uint32_t)b) << 16); }

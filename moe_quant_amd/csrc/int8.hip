@@ -17,8 +17,8 @@ __global__ __launch_bounds__(256) void quantize_tokens_kernel(const void* __rest
   __shared__ float part[4];
   constexpr int KEEP = NV ? NV : 1;
   const int t = threadIdx.x % TPR;
-  const long row = (long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
-  if (TPR < 256 && row >= n) return;
+  const long row = ((long)blockIdx.y * gridDim.x + blockIdx.x) * (256 / TPR) + threadIdx.x / TPR;
+  if (row >= n) return;  // (whole wavefronts, whole workgroups where they meet)
   const void* x0 = (const char*)X + row * ldx * (DT == DT_F32 ? 4 : 2);
   float x[KEEP][8];
   float top = 0.f;
@@ -86,7 +86,7 @@ __global__ __launch_bounds__(256) void quantize_tokens_kernel(const void* __rest
 template <int DT>
 void quantize_launch(const void* X, long ldx, int n, int C, int8_t* Q, long ldq, float* scale, hipStream_t st) {
 #define MQ_QUANT(TPR, NV)                                                                                            \
-  hipLaunchKernelGGL((quantize_tokens_kernel<DT, TPR, NV>), dim3((n + 256 / TPR - 1) / (256 / TPR)), dim3(256), 0, st, X, \
+  hipLaunchKernelGGL((quantize_tokens_kernel<DT, TPR, NV>), mq_wide_grid(((long)n + 256 / TPR - 1) / (256 / TPR)), dim3(256), 0, st, X, \
                      ldx, n, C, Q, ldq, scale)
   if (C <= 512) MQ_QUANT(64, 1);
   else if (C <= 1024) MQ_QUANT(64, 2);
@@ -100,10 +100,12 @@ void quantize_launch(const void* X, long ldx, int n, int C, int8_t* Q, long ldq,
 }
 
 // Rows that start at any byte, copied to rows that start at multiples of 16 (for the tiles).
-__global__ __launch_bounds__(256) void align_rows_kernel(const int8_t* __restrict__ from, long ld, int K, int8_t* __restrict__ to,
-                                                         long ldt) {
-  const int8_t* p = from + (long)blockIdx.x * ld;
-  int8_t* q = to + (long)blockIdx.x * ldt;
+__global__ __launch_bounds__(256) void align_rows_kernel(const int8_t* __restrict__ from, long ld, int n, int K,
+                                                         int8_t* __restrict__ to, long ldt) {
+  const long row = (long)blockIdx.y * gridDim.x + blockIdx.x;
+  if (row >= n) return;
+  const int8_t* p = from + row * ld;
+  int8_t* q = to + row * ldt;
   for (int c = threadIdx.x * 16; c < K; c += 256 * 16) {
     if (c + 16 <= K) {
       intx4 v;
@@ -125,13 +127,13 @@ int int8_dispatch(Int8Args a, int dtype, int swiglu, int8_t* ws, hipStream_t st)
     const long ld = (long)padded(a.K);
     const int rows_b = swiglu ? 2 * a.N : a.N;
     if (!rows_of_words(a.B, a.ldb)) {
-      hipLaunchKernelGGL(align_rows_kernel, dim3(rows_b), dim3(256), 0, st, a.B, a.ldb, a.K, ws, ld);
+      hipLaunchKernelGGL(align_rows_kernel, mq_wide_grid(rows_b), dim3(256), 0, st, a.B, a.ldb, rows_b, a.K, ws, ld);
       a.B = ws;
       a.ldb = ld;
     }
     if (!rows_of_words(a.A, a.lda)) {
       int8_t* to = ws + (size_t)rows_b * ld;
-      hipLaunchKernelGGL(align_rows_kernel, dim3(a.M), dim3(256), 0, st, a.A, a.lda, a.K, to, ld);
+      hipLaunchKernelGGL(align_rows_kernel, mq_wide_grid(a.M), dim3(256), 0, st, a.A, a.lda, a.M, a.K, to, ld);
       a.A = to;
       a.lda = ld;
     }
@@ -159,7 +161,7 @@ constexpr int MAX_K = 131071;  // |sum| <= K 128 128 stays inside 32 bits
 
 extern "C" int mq_quantize_tokens(const void* X, int dtype, long ldx, int n, int C, int8_t* Q, long ldq, float* scale,
                                   void* stream) {
-  if (n < 0 || C <= 0 || ldx < C || ldq < C) return MQ_ERR_ARG;
+  if (n < 0 || C <= 0 || ldx < C || ldq < C || n > MQ_MAX_COUNT || C > MQ_MAX_COUNT) return MQ_ERR_ARG;
   if (!is_dtype(dtype)) return MQ_ERR_ARG;
   if (n == 0) return MQ_OK;
   if (!X || !Q || !scale) return MQ_ERR_ARG;
@@ -176,6 +178,7 @@ extern "C" int mq_matmul_int8(const int8_t* A, long lda, const float* a_scale, c
                               const float* b_scale, const void* bias, void* Y, long ldy, int out_dtype, int M, int N, int K,
                               int swiglu, void* workspace, size_t workspace_bytes, void* stream) {
   if (M < 0 || N <= 0 || K <= 0 || K > MAX_K || lda < K || ldb < K || ldy < N || (swiglu && bias)) return MQ_ERR_ARG;
+  if (M > MQ_MAX_COUNT || N > MQ_MAX_COUNT / 2) return MQ_ERR_ARG;
   if (!is_dtype(out_dtype)) return MQ_ERR_ARG;
   if (M == 0) return MQ_OK;
   if (!A || !a_scale || !B || !b_scale || !Y) return MQ_ERR_ARG;
@@ -191,9 +194,10 @@ extern "C" int mq_matmul_int8_grouped(const int8_t* A, long lda, const float* a_
                                       void* stream) {
   if (S < 0 || E <= 0 || E > 1024 || N <= 0 || K <= 0 || K > MAX_K || lda < K || ldb < K || ldy < N) return MQ_ERR_ARG;
   if (src_rows < 0 || strideB < 0 || (!rows && src_rows < S)) return MQ_ERR_ARG;
+  if (S > MQ_MAX_COUNT || N > MQ_MAX_COUNT / 2) return MQ_ERR_ARG;
   if (!is_dtype(out_dtype)) return MQ_ERR_ARG;
   if (S == 0) return MQ_OK;
-  if (!A || !a_scale || !B || !b_scale || !offsets || !Y) return MQ_ERR_ARG;
+  if (!B || !b_scale || !offsets || !Y || (src_rows > 0 && (!A || !a_scale))) return MQ_ERR_ARG;
   const Int8Args a = {A, lda, a_scale, rows, src_rows, B, ldb, strideB, b_scale, nullptr, Y, ldy, S, N, K, offsets, E, 0};
   return int8_dispatch(a, out_dtype, swiglu, nullptr, (hipStream_t)stream);
 }
@@ -208,6 +212,7 @@ extern "C" int mq_linear_int8(const void* X, int dtype, long ldx, const int8_t* 
                               const void* bias, void* Y, long ldy, int M, int N, int K, void* workspace,
                               size_t workspace_bytes, void* stream) {
   if (M < 0 || N <= 0 || K <= 0 || K > MAX_K || ldx < K || ldb < K || ldy < N || !is_dtype(dtype)) return MQ_ERR_ARG;
+  if (M > MQ_MAX_COUNT || N > MQ_MAX_COUNT / 2) return MQ_ERR_ARG;
   if (M == 0) return MQ_OK;
   if (!X || !B || !b_scale || !Y) return MQ_ERR_ARG;
   hipStream_t st = (hipStream_t)stream;

@@ -773,7 +773,7 @@ int thin_launch(const Int8Args& a, hipStream_t st) {
   // of which would have no rows: 16384 that leave at once take 25 us
   const int by_row = a.offsets && a.M < a.E;
   const long grid = (long)gx * (a.offsets ? min(a.M, a.E) : (a.M + 16 * R - 1) / (16 * R));
-  if (grid > 0x7fffffffL) return MQ_ERR_TOO_LARGE;
+  if (grid * 512 > 0xffffffffL) return MQ_ERR_TOO_LARGE;
   hipLaunchKernelGGL((int8_thin_kernel<DT, SWIGLU, R, C, UN, D>), dim3((unsigned)grid), dim3(512), SMEM, st, a, gx, by_row);
   return mq_check_launch();
 }

@@ -169,10 +169,10 @@ __global__ __launch_bounds__(512) void sort_scatter_kernel(const long* __restric
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void combine_kernel(const void* __restrict__ Y, long ldy, int S, int C,
                                                       const int* __restrict__ slots, const float* __restrict__ weights, int k,
-                                                      void* __restrict__ out, long ldo) {
-  const long t = blockIdx.x;
-  const int c0 = (blockIdx.y * 256 + threadIdx.x) * 8;
-  if (c0 >= C) return;
+                                                      void* __restrict__ out, long ldo, int T) {
+  const long t = (long)blockIdx.y * gridDim.x + blockIdx.x;
+  const int c0 = (blockIdx.z * 256 + threadIdx.x) * 8;
+  if (t >= T || c0 >= C) return;
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   for (int j = 0; j < k; ++j) {
     const int s = slots[t * k + j];
@@ -211,9 +211,9 @@ void combine_launch(const void* Y, long ldy, int S, int C, const int* slots, con
                     long ldo, hipStream_t st) {
   const int per16 = DT == DT_F32 ? 4 : 8;  // elements in 16 bytes
   const bool vec = C % 8 == 0 && ldy % per16 == 0 && ldo % per16 == 0 && ((uintptr_t)Y & 15) == 0 && ((uintptr_t)out & 15) == 0;
-  const dim3 grid(T, (C + 2047) / 2048);
-  if (vec) hipLaunchKernelGGL((combine_kernel<DT, true>), grid, dim3(256), 0, st, Y, ldy, S, C, slots, weights, k, out, ldo);
-  else hipLaunchKernelGGL((combine_kernel<DT, false>), grid, dim3(256), 0, st, Y, ldy, S, C, slots, weights, k, out, ldo);
+  const dim3 grid = mq_wide_grid(T, (C + 2047) / 2048);
+  if (vec) hipLaunchKernelGGL((combine_kernel<DT, true>), grid, dim3(256), 0, st, Y, ldy, S, C, slots, weights, k, out, ldo, T);
+  else hipLaunchKernelGGL((combine_kernel<DT, false>), grid, dim3(256), 0, st, Y, ldy, S, C, slots, weights, k, out, ldo, T);
 }
 
 }  // namespace
@@ -226,6 +226,7 @@ extern "C" int mq_route_experts(const void* logits, int dtype, long ldl, int T, 
   if (n_group <= 0 || n_group > 64 || E % n_group || topk_group <= 0 || topk_group > n_group) return MQ_ERR_ARG;
   if (group_top < 1 || group_top > 2 || group_top > E / n_group || (long)topk_group * (E / n_group) < top_k) return MQ_ERR_ARG;
   if (dtype != DT_F32 && dtype != DT_BF16 && dtype != DT_F16) return MQ_ERR_ARG;
+  if (T > 1 << 25) return MQ_ERR_TOO_LARGE;  // 64 threads a row at most, fewer than 2^32 in all
   if (T == 0) return MQ_OK;
   if (!logits || !weights || !ids) return MQ_ERR_ARG;
   RouteArgs a = {logits, ldl, T, E, top_k, score, bias, n_group, topk_group, group_top, renormalize, scale, weights, ids, 0, 0, 0, 0};
@@ -268,7 +269,7 @@ extern "C" int mq_sort_by_expert(const long* ids, int T, int top_k, int E, long*
 
 extern "C" int mq_combine_experts(const void* Y, int dtype, long ldy, int S, int C, const int* slots, const float* weights,
                                   int T, int k, void* out, long ldo, void* stream) {
-  if (S < 0 || C <= 0 || T < 0 || k <= 0 || ldy < C || ldo < C) return MQ_ERR_ARG;
+  if (S < 0 || C <= 0 || T < 0 || k <= 0 || ldy < C || ldo < C || T > MQ_MAX_COUNT || C > 1 << 26) return MQ_ERR_ARG;
   if (dtype != DT_F32 && dtype != DT_BF16 && dtype != DT_F16) return MQ_ERR_ARG;
   if (T == 0) return MQ_OK;
   if (!slots || !weights || !out || (S > 0 && !Y)) return MQ_ERR_ARG;

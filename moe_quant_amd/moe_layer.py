@@ -116,9 +116,13 @@ def experts_forward_int8(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tens
     (T, top_k) int64 and weights (T, top_k) fp32 as a `Router` gives them (ids outside the experts add nothing).  Tokens and
     the product between the projections, held in x's type, are quantized to 8 bits with a scale per row.  Nothing is read
     back to the host."""
+    if experts.gate_up.dim() != 3 or experts.down.dim() != 3:
+        raise ValueError("gate_up must be (E, 2 I, C) and down (E, C, I)")
     E, C = experts.gate_up.shape[0], experts.gate_up.shape[2]
     if x.dim() != 2 or x.shape[1] != C or ids.shape != weights.shape or ids.dim() != 2 or ids.shape[0] != x.shape[0]:
         raise ValueError("x must be (T, C) with the experts' C, ids and weights (T, top_k)")
+    if experts.gate_up.shape[1] % 2 or experts.down.shape != (E, C, experts.gate_up.shape[1] // 2):
+        raise ValueError("gate_up must be (E, 2 I, C) and down (E, C, I)")
     rows, offsets, slots = ops.sort_by_expert(ids, E)
     codes, scale = ops.quantize_tokens(x)
     h = ops.matmul_int8_grouped(codes, scale, experts.gate_up, experts.gate_up_scale, offsets, rows, x.dtype, swiglu=True)

@@ -651,6 +651,12 @@ def _rows(X: Tensor) -> Tuple[Tensor, int]:
     return X, (X.stride(0) if n > 1 else C)
 
 
+def _fits(*counts: int) -> None:
+    """Row and column counts reach the library as 32-bit integers, with room to round one up to a tile."""
+    if max(counts) > (1 << 30):
+        raise ValueError("at most 2^30 rows or columns")
+
+
 _SCORES = {"softmax": 0, "sigmoid": 1}
 
 
@@ -667,6 +673,8 @@ def route_experts(logits: Tensor, top_k: int, *, score: str = "softmax", bias: O
     if logits.dim() != 2 or logits.dtype not in _DT:
         raise ValueError("logits must be (T, E) fp32, bf16 or fp16")
     T, E = logits.shape
+    if T > 1 << 25:
+        raise ValueError("at most 2^25 rows of logits a call")
     if score not in _SCORES:
         raise ValueError(f"score must be 'softmax' or 'sigmoid', got {score!r}")
     if not 1 <= E <= 1024 or not 1 <= top_k <= min(E, 64):
@@ -730,6 +738,7 @@ def combine_experts(Y: Tensor, slots: Tensor, weights: Tensor) -> Tensor:
         raise ValueError("slots must be (T, k) int32")
     if weights.shape != slots.shape or weights.dtype != torch.float32:
         raise ValueError("weights must be fp32 of the shape of slots")
+    _fits(Y.shape[0], slots.shape[0], slots.shape[1], 16 * Y.shape[1])
     with _on(Y, slots, weights):
         Y, ldy = _rows(Y)
         slots, weights = slots.contiguous(), weights.contiguous()
@@ -751,6 +760,7 @@ def quantize_tokens(X: Tensor) -> Tuple[Tensor, Tensor]:
     scale NaN (its products are NaN, no other row's)."""
     if X.dim() != 2 or X.dtype not in _DT or X.shape[1] < 1:
         raise ValueError("X must be (n, C) fp32, bf16 or fp16")
+    _fits(*X.shape)
     with _on(X):
         X, ldx = _rows(X)
         n, C = X.shape
@@ -778,6 +788,7 @@ def _int8_operands(A, a_scale, B, b_scale, out_dtype, swiglu) -> int:
     rows = B.shape[-2]
     if rows < 1 or (swiglu and rows % 2):
         raise ValueError("B needs at least one row, and gate and up halves of equal length with swiglu")
+    _fits(A.shape[0], rows)
     return rows // 2 if swiglu else rows
 
 
@@ -813,6 +824,7 @@ def linear_int8(X: Tensor, B: Tensor, b_scale: Tensor, bias: Optional[Tensor] = 
     if B.dim() != 2 or B.dtype != torch.int8 or B.shape[1] != K or not 1 <= K <= _MAX_K or B.shape[0] < 1:
         raise ValueError(f"B must be (N, K) int8 with X's K columns, 1 <= K <= {_MAX_K}")
     N = B.shape[0]
+    _fits(X.shape[0], N)
     if b_scale.dtype != torch.float32 or b_scale.shape != (N,) or not b_scale.is_contiguous():
         raise ValueError("b_scale must be contiguous fp32, one value per row of B")
     if bias is not None and (bias.dtype != X.dtype or bias.shape != (N,) or not bias.is_contiguous()):
@@ -848,19 +860,21 @@ def matmul_int8_grouped(A: Tensor, a_scale: Tensor, B: Tensor, b_scale: Tensor, 
     if rows is not None and (rows.dtype != torch.int64 or rows.dim() != 1 or not rows.is_contiguous()):
         raise ValueError("rows must be a contiguous int64 vector")
     S = A.shape[0] if rows is None else rows.numel()
+    _fits(S, 1)
     if out is not None and (out.shape != (S, N) or out.dtype != out_dtype or (N > 1 and out.stride(1) != 1)
                             or (S > 1 and out.stride(0) < N)):
         raise ValueError("out must be (S, N) of out_dtype with unit column stride")
     with _on(A, a_scale, B, b_scale, offsets, rows, out):
         A, lda = _rows(A)
-        if B.stride(2) != 1 or B.stride(1) < B.shape[2] or B.stride(0) < 0:
+        K = B.shape[2]
+        if (K > 1 and B.stride(2) != 1) or (B.shape[1] > 1 and B.stride(1) < K):
             B = B.contiguous()
         if out is None:
             out = torch.empty(S, N, dtype=out_dtype, device=A.device)
         rc = _lib.load().mq_matmul_int8_grouped(
-            A.data_ptr(), lda, a_scale.data_ptr(), A.shape[0], _p(rows), S, B.data_ptr(), B.stride(1), B.stride(0),
-            b_scale.data_ptr(), E, offsets.data_ptr(), out.data_ptr(), out.stride(0) if S > 1 else N, _DT[out_dtype], N,
-            A.shape[1], int(swiglu), _stream(A))
+            A.data_ptr(), lda, a_scale.data_ptr(), A.shape[0], _p(rows), S, B.data_ptr(),
+            B.stride(1) if B.shape[1] > 1 else K, B.stride(0), b_scale.data_ptr(), E, offsets.data_ptr(), out.data_ptr(),
+            out.stride(0) if S > 1 else N, _DT[out_dtype], N, K, int(swiglu), _stream(A))
     check(rc, "mq_matmul_int8_grouped")
     return out
 

@@ -500,6 +500,97 @@ def test_grouped_strange_offsets(dev):
     _close(out[20:, 16:48], want, mag, None, torch.float32)
 
 
+def test_grouped_strange_offsets_few_rows(dev):
+    """The same with fewer rows than experts (rows look their experts up), and rows that leave A altogether."""
+    g = _gen(15)
+    E, S = 70, 9
+    A, B = _rand_codes(g, S, 64), _rand_codes(g, E, 32, 64)
+    sa, sb = torch.ones(S), torch.ones(E, 32)
+    up = torch.arange(E + 1)
+    for off in (up * 0, up * 0 + S, up - 30, up.flip(0), torch.where(up > 40, up * 0 + 5, up * 0), up * 2**35 - 2**36):
+        frame = torch.full((S + 20, 32), 5.0, device=dev)
+        out = frame[10:10 + S]
+        ops.matmul_int8_grouped(A.to(dev), sa.to(dev), B.to(dev), sb.to(dev), off.to(dev), None, torch.float32, False, out)
+        assert (frame[:10] == 5).all() and (frame[10 + S:] == 5).all()
+    off = torch.where(up > 40, up * 0 + S, up * 0)  # all rows belong to expert 40
+    for rows in (None, torch.tensor([-1, 9, 2**40, -2**50, 0, 8, 3, 3, 9])):
+        got = ops.matmul_int8_grouped(A.to(dev), sa.to(dev), B.to(dev), sb.to(dev), off.to(dev),
+                                      None if rows is None else rows.to(dev), torch.float32)
+        took = A if rows is None else torch.stack([A[r] if 0 <= r < S else A[0] * 0 for r in rows.tolist()])
+        assert torch.equal(got.cpu().double(), took.double() @ B[40].double().t())
+    for n in (S, 700):  # no rows in A at all: without tiles and with them
+        off = torch.where(up > 40, up * 0 + n, up * 0)
+        none = ops.matmul_int8_grouped(A.to(dev)[:0], sa.to(dev)[:0], B.to(dev), sb.to(dev), off.to(dev),
+                                       torch.zeros(n, dtype=torch.int64, device=dev), torch.float32)
+        assert none.shape == (n, 32) and (none == 0).all()
+
+
+@pytest.mark.parametrize("dt,K,swiglu,gather", [("bf16", 64, False, False), ("f16", 449, True, True), ("f32", 204, False, True)])
+def test_grouped_many_rows(dev, dt, K, swiglu, gather):
+    """Large tiles: many rows an expert, and enough tiles to go round several times."""
+    g, dt = _gen(K), DT[dt]
+    counts, N, ld = [600, 0, 300, 260, 5, 1000], 18708, (K + 3) // 4 * 4
+    E, S = len(counts), sum(counts)
+    offsets = torch.tensor([0] + list(torch.tensor(counts).cumsum(0)))
+    B = _rand_codes(g, E, N, ld)
+    sb = (torch.rand(E, N, generator=g) + 0.1) / (100 * K**0.5)
+    A, sa = _rand_codes(g, S, ld), torch.rand(S, generator=g) + 0.1
+    rows = torch.randint(0, S, (S,), generator=g) if gather else torch.arange(S)
+    if gather:
+        rows[0], rows[601], rows[S - 1] = -1, S, 2**40
+    out = torch.full((S + 3, N // 2 if swiglu else N), 77.0, dtype=dt, device=dev)
+    ops.matmul_int8_grouped(A.to(dev)[:, :K], sa.to(dev), B.to(dev)[:, :, :K], sb.to(dev), offsets.to(dev),
+                            rows.to(dev) if gather else None, dt, swiglu, out[:S])
+    out = out.cpu()
+    assert (out[S:] == 77).all()
+    live = (rows >= 0) & (rows < S)
+    took = torch.where(live, rows, torch.zeros_like(rows))
+    for e in range(E):
+        lo, hi = offsets[e], offsets[e + 1]
+        for c in range(lo, hi, 256):  # (parts, to keep the 64-bit results small)
+            d = min(c + 256, hi)
+            r = took[c:d]
+            want, mag, extra = _product64(A[r, :K] * live[c:d, None].to(torch.int8), sa[r], B[e, :, :K], sb[e], None, swiglu)
+            _close(out[c:d], want, mag, extra, dt)
+
+
+def test_grouped_one_row_of_weights(dev):
+    g = _gen(16)
+    full = _rand_codes(g, 4, 3, 96)
+    A, sa = _rand_codes(g, 30, 96), torch.rand(30, generator=g)
+    off = torch.tensor([0, 7, 7, 20, 30])
+    sb = torch.rand(4, 1, generator=g)
+    got = ops.matmul_int8_grouped(A.to(dev), sa.to(dev), full.to(dev)[:, 1:2], sb.to(dev), off.to(dev), None, torch.float32)
+    for e in range(4):
+        lo, hi = off[e], off[e + 1]
+        if lo < hi:
+            want, mag, _ = _product64(A[lo:hi], sa[lo:hi], full[e, 1:2], sb[e])
+            _close(got[lo:hi], want, mag, None, torch.float32)
+
+
+def test_experts_forward_without_tokens(dev):
+    ex = _experts(_gen(17), 4, 64, 16, dev)
+    y = moe_layer.experts_forward_int8(torch.zeros(0, 64, device=dev), torch.zeros(0, 2, dtype=torch.int64, device=dev),
+                                       torch.zeros(0, 2, device=dev), ex)
+    assert y.shape == (0, 64)
+    x = torch.randn(3, 64, device=dev)
+    nobody = torch.full((3, 2), -1, dtype=torch.int64, device=dev)  # every choice dropped
+    assert (moe_layer.experts_forward_int8(x, nobody, torch.ones(3, 2, device=dev), ex) == 0).all()
+
+
+def test_rows_beyond_one_grid_dimension(dev):
+    """More than 65536 workgroups of one row each."""
+    x = torch.randn(70001, 1040, generator=_gen(18)).bfloat16()
+    q, s = ops.quantize_tokens(x.to(dev))
+    want, ws = _codes64(x)
+    assert torch.equal(q.cpu(), want) and ((s.cpu().double() - ws).abs() <= U * ws).all()
+    Y = torch.randn(50, 16, generator=_gen(19))
+    slots = torch.randint(0, 50, (140001, 1), generator=_gen(20), dtype=torch.int32)
+    w = torch.rand(140001, 1, generator=_gen(21))
+    out = ops.combine_experts(Y.to(dev), slots.to(dev), w.to(dev)).cpu()
+    assert torch.equal(out, Y[slots[:, 0].long()] * w)
+
+
 def test_grouped_weights_with_gaps(dev):
     g = _gen(6)
     full = _rand_codes(g, 6, 80, 160)

@@ -195,3 +195,40 @@ def test_route_tokens_on_the_host_is_unchanged():
     ids = torch.tensor([[2, 0], [1, 2], [0, 1]])
     rows, offsets = moe_layer.route_tokens(ids, 4)
     assert rows.tolist() == [0, 2, 1, 2, 0, 1] and offsets == [0, 2, 4, 6, 6]
+
+
+def test_counts_beyond_32_bits_are_refused():
+    """Sizes that a 32-bit count would cut: refused before anything is launched (the tensors are one element each)."""
+    huge = torch.zeros(1, dtype=I8).expand((1 << 30) + 1, 64)
+    small = torch.zeros(8, 64, dtype=I8)
+    many = torch.zeros(1).expand((1 << 30) + 1)
+    with pytest.raises(ValueError):
+        ops.quantize_tokens(torch.zeros(1).expand((1 << 30) + 1, 4))
+    with pytest.raises(ValueError):
+        ops.matmul_int8(huge, many, small, torch.zeros(8))
+    with pytest.raises(ValueError):
+        ops.linear_int8(torch.zeros(1).expand((1 << 32) + 1, 64), small, torch.zeros(8))
+    with pytest.raises(ValueError):
+        ops.route_experts(torch.zeros(1).expand((1 << 25) + 1, 8), 2)
+    with pytest.raises(ValueError):
+        ops.combine_experts(torch.zeros(1).expand(4, 1 << 27), torch.zeros(1, 1, dtype=I32), torch.zeros(1, 1))
+    lib = _lib.load()
+    p = ctypes.cast(ctypes.create_string_buffer(64), ctypes.c_void_p)
+    top = 0x7fffffff
+    assert lib.mq_quantize_tokens(p, 0, 8, top, 8, p, 8, p, None) == _lib.MQ_ERR_ARG
+    assert lib.mq_matmul_int8(p, 32, p, p, 32, p, None, p, 8, 1, top, 8, 32, 0, None, 0, None) == _lib.MQ_ERR_ARG
+    assert lib.mq_linear_int8(p, 0, 32, p, 32, p, None, p, 8, top, 8, 32, p, 1 << 40, None) == _lib.MQ_ERR_ARG
+    assert lib.mq_matmul_int8_grouped(p, 32, p, top, None, top, p, 32, 256, p, 2, p, p, 8, 1, 8, 32, 0, None) == _lib.MQ_ERR_ARG
+    assert lib.mq_combine_experts(p, 0, 8, 4, 8, p, p, top, 2, p, 8, None) == _lib.MQ_ERR_ARG
+    assert lib.mq_route_experts(p, 0, 16, top, 16, 2, 0, None, 1, 1, 1, 1, 1.0, p, p, None) == _lib.MQ_ERR_TOO_LARGE
+
+
+def test_experts_forward_refusals():
+    z = lambda *s: torch.zeros(*s, dtype=I8)
+    ex = moe_layer.Int8Experts(z(3, 8, 16), torch.zeros(3, 8), z(3, 16, 4), torch.zeros(3, 16))
+    x, ids, w = torch.zeros(5, 16), torch.zeros(5, 2, dtype=I64), torch.zeros(5, 2)
+    for bad in ((x[:, :8], ids, w, ex), (x[0], ids, w, ex), (x, ids[:4], w, ex), (x, ids, w[:, :1], ex), (x, ids[:, 0], w[:, 0], ex),
+                (x, ids, w, moe_layer.Int8Experts(z(3, 8, 16), torch.zeros(3, 8), z(3, 15, 4), torch.zeros(3, 15))),
+                (x, ids, w, moe_layer.Int8Experts(z(8, 16), torch.zeros(8), z(16, 4), torch.zeros(16)))):
+        with pytest.raises(ValueError):
+            moe_layer.experts_forward_int8(*bad)
