@@ -336,6 +336,12 @@ __global__ __launch_bounds__(256, 6) void route_kernel(RouteArgs a) {
   }
   if (a.n_group > 1) {
     const int per = a.E / a.n_group;
+    // the two best of a group may cancel (large biases of both signs): then the sum's error is not small against the sum
+    bool unsure = false;
+    const auto sum = [&](float best, float second) {
+      unsure |= fabsf(best) + fabsf(second) > 4.f * fabsf(best + second) + 4.f;
+      return best + second;
+    };
     if (a.group_lanes) {
       // a group is a run of 1, 2, 4, 8 or 16 lanes' chunks: exchanges with the lane 1, 2, 4, 8 away (mirrors do for the last
       // two: the quads, then the halves, agree by then)
@@ -355,7 +361,7 @@ __global__ __launch_bounds__(256, 6) void route_kernel(RouteArgs a) {
         if (a.group_lanes >= 16) MQ_MEET(0x140);
 #undef MQ_MEET
         const int at = j + L * i;
-        if ((at & (a.group_lanes - 1)) == 0 && 4 * at < a.E) gs[slot][at >> a.group_shift] = a.group_top == 2 ? best + second : best;
+        if ((at & (a.group_lanes - 1)) == 0 && 4 * at < a.E) gs[slot][at >> a.group_shift] = a.group_top == 2 ? sum(best, second) : best;
       }
     } else {
 #pragma unroll
@@ -372,12 +378,11 @@ __global__ __launch_bounds__(256, 6) void route_kernel(RouteArgs a) {
           best = fmaxf(best, x);
           at = at + 1 == per ? 0 : at + 1;
         }
-        gs[slot][g] = a.group_top == 2 ? best + second : best;
+        gs[slot][g] = a.group_top == 2 ? sum(best, second) : best;
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     unsigned kept = 0;
-    bool unsure = false;
     for (int g = j, n = 0; g < a.n_group; g += L, ++n) {
       const float mine = gs[slot][g], near = 0x1p-18f + fabsf(mine) * 0x1p-20f;
       int sure = 0, maybe = 0;

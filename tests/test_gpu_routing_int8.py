@@ -110,6 +110,17 @@ def test_route_groups(dev, dtype, score, group_top):
 
 
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_groups_whose_best_cancel(dev, score):
+    """Biases of both signs, so that a group's two best almost cancel: their sum is what tells the groups apart."""
+    for T, E, k, G, tg in [(40, 64, 4, 8, 3), (40, 60, 3, 4, 2), (17, 256, 8, 8, 4), (9, 1024, 16, 16, 5)]:
+        _say("cancel", T, E, k, G, tg, score)
+        logits = 2 * torch.randn(T, E, generator=_gen(T + E))
+        bias = torch.full((G, E // G), -(2.0**20))
+        bias[:, 3] = 2.0**20
+        _check_route(dev, logits, k, score=score, bias=bias.reshape(-1).to(dev), n_group=G, topk_group=tg)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_route_ties_and_near_ties(dev, score):
     """Equal logits everywhere, equal pairs, and neighbours one 32-bit step apart, with and without a bias."""
     E = 256
