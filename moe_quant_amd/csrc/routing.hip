@@ -256,7 +256,7 @@ extern "C" int mq_sort_by_expert(const long* ids, int T, int top_k, int E, long*
                        offsets, slots);
     return mq_check_launch();
   }
-  if (!workspace || workspace_bytes < mq_sort_by_expert_workspace_bytes(T, top_k, E)) return MQ_ERR_WORKSPACE;
+  if (!workspace || workspace_bytes < mq_sort_by_expert_workspace_bytes(T, top_k, E) || ((uintptr_t)workspace & 3)) return MQ_ERR_WORKSPACE;
   const int blocks = (n + SORT_CHUNK - 1) / SORT_CHUNK;
   int* total = reinterpret_cast<int*>(workspace);
   int* count = total + E + 1;

@@ -232,3 +232,13 @@ def test_experts_forward_refusals():
                 (x, ids, w, moe_layer.Int8Experts(z(8, 16), torch.zeros(8), z(16, 4), torch.zeros(16)))):
         with pytest.raises(ValueError):
             moe_layer.experts_forward_int8(*bad)
+
+
+def test_sort_workspace_alignment():
+    lib = _lib.load()
+    buf = ctypes.create_string_buffer(64)
+    p = ctypes.cast(buf, ctypes.c_void_p)
+    need = lib.mq_sort_by_expert_workspace_bytes(10000, 1, 4)
+    for off in (1, 2, 3):
+        at = ctypes.c_void_p((p.value + 3) // 4 * 4 + off)
+        assert lib.mq_sort_by_expert(p, 10000, 1, 4, p, p, p, at, need, None) == _lib.MQ_ERR_WORKSPACE
