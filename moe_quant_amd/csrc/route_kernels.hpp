@@ -457,7 +457,7 @@ __global__ __launch_bounds__(256, 6) void route_kernel(RouteArgs a) {
   sort_down<V>(key);
 
   uint32_t last = 0, kth = 0;
-  int popped = 0;
+  int popped = 0, found = 0;  // candidates this lane gave up; rounds that found one, the same in all of the row's lanes
   bool near = false;
 #pragma unroll
   for (int r = 0; r <= KT; ++r) {
@@ -474,6 +474,7 @@ __global__ __launch_bounds__(256, 6) void route_kernel(RouteArgs a) {
     }
     if (r < a.top_k) kth = best;
     last = best;
+    found += best != 0;
     if (mine) {
       ++popped;
       if (r < a.top_k) {
@@ -485,8 +486,10 @@ __global__ __launch_bounds__(256, 6) void route_kernel(RouteArgs a) {
       if (V <= KT - r) key[V - 1] = 0;
     }
   }
-  // equal keys in two lanes leave together: then more have been taken than rounds were run
-  if (!sure_keys) near |= row_sum<L>((float)popped) > (float)(a.top_k + 1);
+  // equal keys in two lanes leave together, with one place of `res` for both: then more candidates have left than rounds found
+  // one.  (Not more than top_k + 1: where hardly more than top_k candidates exist, the last rounds find none.)  Without such
+  // keys every round before the last has found one, since at least top_k candidates exist, and every place is written.
+  if (!sure_keys) near |= row_sum<L>((float)popped) > (float)found;
 
   const unsigned long my_row = L == 64 ? ~0ul : ((1ul << (L & 63)) - 1) << (L * sub);
   if (__ballot(near)) {
@@ -543,7 +546,7 @@ __global__ __launch_bounds__(256, 6) void route_kernel(RouteArgs a) {
   float w = 0.f;
   int e = 0;
   if (j < a.top_k) {
-    e = min(max(res[slot][j], 0), a.E - 1);  // (a slow row may have left a place empty)
+    e = min(max(res[slot][j], 0), a.E - 1);  // (a slow row may have left a place empty: it is routed again below)
     const float x = load_val<DT>(a.logits, base + e);
     if (sigmoid) {
       w = 1.f / (1.f + __expf(-x));
