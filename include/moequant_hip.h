@@ -337,6 +337,10 @@ int mq_sort_by_expert(const long* ids, int T, int top_k, int E, long* rows, long
  * [0, S) add nothing.  Y : S x C (ldy), out : T x C (ldo), both of type dtype; out must not overlap Y.  C <= 2^26. */
 int mq_combine_experts(const void* Y, int dtype, long ldy, int S, int C, const int* slots, const float* weights, int T, int k,
                        void* out, long ldo, void* stream);
+/* The same from fp32 Y to out of out_dtype, so that the experts' outputs are rounded once, after the sum (any other Y: out_dtype
+ * must be its dtype). */
+int mq_combine_experts_to(const void* Y, int dtype, long ldy, int S, int C, const int* slots, const float* weights, int T, int k,
+                          void* out, int out_dtype, long ldo, void* stream);
 
 /* ---- (6) products on 8-bit integers ----------------------------------------------------------------------------
  * Row and column counts stay below 2^31 - 4096 (weights' rows below half of that).

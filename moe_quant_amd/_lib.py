@@ -57,6 +57,7 @@ SIGNATURES = {
     "mq_sort_by_expert_workspace_bytes": (_sz, [_i, _i, _i]),
     "mq_sort_by_expert": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
     "mq_combine_experts": (_i, [_vp, _i, _l, _i, _i, _vp, _vp, _i, _i, _vp, _l, _vp]),
+    "mq_combine_experts_to": (_i, [_vp, _i, _l, _i, _i, _vp, _vp, _i, _i, _vp, _i, _l, _vp]),
     "mq_quantize_tokens": (_i, [_vp, _i, _l, _i, _i, _vp, _l, _vp, _vp]),
     "mq_matmul_int8_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "mq_matmul_int8": (_i, [_vp, _l, _vp, _vp, _l, _vp, _vp, _vp, _l, _i, _i, _i, _i, _i, _vp, _sz, _vp]),

@@ -3,7 +3,7 @@
 //
 //   mq_route_experts   : logits -> the top_k experts of each token and their weights
 //   mq_sort_by_expert  : expert ids -> token rows in expert order, offsets, and each choice's position in that order
-//   mq_combine_experts : out[t] = sum_j weight[t, j] * Y[slot[t, j]]
+//   mq_combine_experts : out[t] = sum_j weight[t, j] * Y[slot[t, j]] (_to: in another type than Y's)
 #include "common.hpp"
 #include "route_kernels.hpp"
 
@@ -164,9 +164,9 @@ __global__ __launch_bounds__(512) void sort_scatter_kernel(const long* __restric
 
 // ---- combine --------------------------------------------------------------------------------------------
 // One workgroup per (token, 2048 columns); the sum runs in the order of the token's choices, in 32 bits, and is rounded
-// once.  Slots outside [0, S) add nothing.  Bound by memory: 220 us for 8192 tokens of eight experts, 7168 bf16 columns (4.8
-// TB/s).
-template <int DT, bool VEC>
+// once, to the type TO of the results.  Slots outside [0, S) add nothing.  Bound by memory: 220 us for 8192 tokens of eight
+// experts, 7168 bf16 columns (4.8 TB/s).
+template <int DT, int TO, bool VEC>
 __global__ __launch_bounds__(256) void combine_kernel(const void* __restrict__ Y, long ldy, int S, int C,
                                                       const int* __restrict__ slots, const float* __restrict__ weights, int k,
                                                       void* __restrict__ out, long ldo, int T) {
@@ -200,20 +200,20 @@ __global__ __launch_bounds__(256) void combine_kernel(const void* __restrict__ Y
 #pragma unroll
   for (int e = 0; e < 8; ++e)
     if (VEC || c0 + e < C) {
-      if (DT == DT_F32) ((float*)out)[to + e] = acc[e];
-      else if (DT == DT_BF16) ((uint16_t*)out)[to + e] = f32_to_bf16_bits(acc[e]);
+      if (TO == DT_F32) ((float*)out)[to + e] = acc[e];
+      else if (TO == DT_BF16) ((uint16_t*)out)[to + e] = f32_to_bf16_bits(acc[e]);
       else ((_Float16*)out)[to + e] = (_Float16)acc[e];
     }
 }
 
-template <int DT>
+template <int DT, int TO>
 void combine_launch(const void* Y, long ldy, int S, int C, const int* slots, const float* weights, int T, int k, void* out,
                     long ldo, hipStream_t st) {
-  const int per16 = DT == DT_F32 ? 4 : 8;  // elements in 16 bytes
-  const bool vec = C % 8 == 0 && ldy % per16 == 0 && ldo % per16 == 0 && ((uintptr_t)Y & 15) == 0 && ((uintptr_t)out & 15) == 0;
+  constexpr int PER16 = DT == DT_F32 ? 4 : 8, PER16_TO = TO == DT_F32 ? 4 : 8;  // elements in 16 bytes
+  const bool vec = C % 8 == 0 && ldy % PER16 == 0 && ldo % PER16_TO == 0 && ((uintptr_t)Y & 15) == 0 && ((uintptr_t)out & 15) == 0;
   const dim3 grid = mq_wide_grid(T, (C + 2047) / 2048);
-  if (vec) hipLaunchKernelGGL((combine_kernel<DT, true>), grid, dim3(256), 0, st, Y, ldy, S, C, slots, weights, k, out, ldo, T);
-  else hipLaunchKernelGGL((combine_kernel<DT, false>), grid, dim3(256), 0, st, Y, ldy, S, C, slots, weights, k, out, ldo, T);
+  if (vec) hipLaunchKernelGGL((combine_kernel<DT, TO, true>), grid, dim3(256), 0, st, Y, ldy, S, C, slots, weights, k, out, ldo, T);
+  else hipLaunchKernelGGL((combine_kernel<DT, TO, false>), grid, dim3(256), 0, st, Y, ldy, S, C, slots, weights, k, out, ldo, T);
 }
 
 }  // namespace
@@ -267,15 +267,25 @@ extern "C" int mq_sort_by_expert(const long* ids, int T, int top_k, int E, long*
   return mq_check_launch();
 }
 
-extern "C" int mq_combine_experts(const void* Y, int dtype, long ldy, int S, int C, const int* slots, const float* weights,
-                                  int T, int k, void* out, long ldo, void* stream) {
+extern "C" int mq_combine_experts_to(const void* Y, int dtype, long ldy, int S, int C, const int* slots, const float* weights,
+                                     int T, int k, void* out, int out_dtype, long ldo, void* stream) {
   if (S < 0 || C <= 0 || T < 0 || k <= 0 || ldy < C || ldo < C || T > MQ_MAX_COUNT || C > 1 << 26) return MQ_ERR_ARG;
   if (dtype != DT_F32 && dtype != DT_BF16 && dtype != DT_F16) return MQ_ERR_ARG;
+  if (out_dtype != dtype && (dtype != DT_F32 || (out_dtype != DT_BF16 && out_dtype != DT_F16))) return MQ_ERR_ARG;
   if (T == 0) return MQ_OK;
   if (!slots || !weights || !out || (S > 0 && !Y)) return MQ_ERR_ARG;
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == DT_F32) combine_launch<DT_F32>(Y, ldy, S, C, slots, weights, T, k, out, ldo, st);
-  else if (dtype == DT_BF16) combine_launch<DT_BF16>(Y, ldy, S, C, slots, weights, T, k, out, ldo, st);
-  else combine_launch<DT_F16>(Y, ldy, S, C, slots, weights, T, k, out, ldo, st);
+#define MQ_COMBINE(DT, TO) combine_launch<DT, TO>(Y, ldy, S, C, slots, weights, T, k, out, ldo, st)
+  if (dtype == DT_BF16) MQ_COMBINE(DT_BF16, DT_BF16);
+  else if (dtype == DT_F16) MQ_COMBINE(DT_F16, DT_F16);
+  else if (out_dtype == DT_BF16) MQ_COMBINE(DT_F32, DT_BF16);
+  else if (out_dtype == DT_F16) MQ_COMBINE(DT_F32, DT_F16);
+  else MQ_COMBINE(DT_F32, DT_F32);
+#undef MQ_COMBINE
   return mq_check_launch();
+}
+
+extern "C" int mq_combine_experts(const void* Y, int dtype, long ldy, int S, int C, const int* slots, const float* weights,
+                                  int T, int k, void* out, long ldo, void* stream) {
+  return mq_combine_experts_to(Y, dtype, ldy, S, C, slots, weights, T, k, out, dtype, ldo, stream);
 }

@@ -115,8 +115,9 @@ def experts_forward_int8(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tens
     """The expert part of a block's forward on its quantized weights:
     y[t] = sum_j weights[t, j] * down_e(silu(gate_e(x[t])) * up_e(x[t])), e = ids[t, j].  x (T, C) fp32, bf16 or fp16; ids
     (T, top_k) int64 and weights (T, top_k) fp32 as a `Router` gives them (ids outside the experts add nothing).  Tokens and
-    the product between the projections, held in x's type, are quantized to 8 bits with a scale per row.  Nothing is read
-    back to the host."""
+    the product between the projections, held in x's type, are quantized to 8 bits with a scale per row; the experts' outputs
+    are fp32 (T * top_k * C values of scratch memory) and rounded once, after their weighted sum.  Nothing is read back to
+    the host."""
     if experts.gate_up.dim() != 3 or experts.down.dim() != 3:
         raise ValueError("gate_up must be (E, 2 I, C) and down (E, C, I)")
     E, C = experts.gate_up.shape[0], experts.gate_up.shape[2]
@@ -128,8 +129,8 @@ def experts_forward_int8(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tens
     codes, scale = ops.quantize_tokens(x)
     h = ops.matmul_int8_grouped(codes, scale, experts.gate_up, experts.gate_up_scale, offsets, rows, x.dtype, swiglu=True)
     codes, scale = ops.quantize_tokens(h)
-    y = ops.matmul_int8_grouped(codes, scale, experts.down, experts.down_scale, offsets, None, x.dtype)
-    return ops.combine_experts(y, slots, weights)
+    y = ops.matmul_int8_grouped(codes, scale, experts.down, experts.down_scale, offsets, None, torch.float32)
+    return ops.combine_experts(y, slots, weights, x.dtype)
 
 
 @torch.no_grad()

@@ -728,25 +728,28 @@ def sort_by_expert(ids: Tensor, n_experts: int) -> Tuple[Tensor, Tensor, Tensor]
     return rows, offsets, slots
 
 
-def combine_experts(Y: Tensor, slots: Tensor, weights: Tensor) -> Tensor:
+def combine_experts(Y: Tensor, slots: Tensor, weights: Tensor, out_dtype: Optional[torch.dtype] = None) -> Tensor:
     """out[t] = sum_j weights[t, j] * Y[slots[t, j]]: the experts' outputs Y (S, C) fp32/bf16/fp16 (rows in expert order)
-    back to tokens, out (T, C) of Y's type.  slots (T, k) int32 from `sort_by_expert` (outside [0, S): adds nothing),
-    weights (T, k) fp32.  Summed in fp32 in the order of j, rounded once."""
+    back to tokens, out (T, C) of Y's type or, for fp32 Y, of out_dtype.  slots (T, k) int32 from `sort_by_expert` (outside
+    [0, S): adds nothing), weights (T, k) fp32.  Summed in fp32 in the order of j, rounded once."""
     if Y.dim() != 2 or Y.dtype not in _DT or Y.shape[1] < 1:
         raise ValueError("Y must be (S, C) fp32, bf16 or fp16")
     if slots.dim() != 2 or slots.dtype != torch.int32 or slots.shape[1] < 1:
         raise ValueError("slots must be (T, k) int32")
     if weights.shape != slots.shape or weights.dtype != torch.float32:
         raise ValueError("weights must be fp32 of the shape of slots")
+    out_dtype = Y.dtype if out_dtype is None else out_dtype
+    if out_dtype not in _DT or (out_dtype != Y.dtype and Y.dtype != torch.float32):
+        raise ValueError("out_dtype must be Y's type, or fp32, bf16 or fp16 where Y is fp32")
     _fits(Y.shape[0], slots.shape[0], slots.shape[1], 16 * Y.shape[1])
     with _on(Y, slots, weights):
         Y, ldy = _rows(Y)
         slots, weights = slots.contiguous(), weights.contiguous()
         (S, C), (T, k) = Y.shape, slots.shape
-        out = torch.empty(T, C, dtype=Y.dtype, device=Y.device)
-        rc = _lib.load().mq_combine_experts(Y.data_ptr(), _DT[Y.dtype], ldy, S, C, slots.data_ptr(), weights.data_ptr(), T, k,
-                                            out.data_ptr(), C, _stream(Y))
-    check(rc, "mq_combine_experts")
+        out = torch.empty(T, C, dtype=out_dtype, device=Y.device)
+        rc = _lib.load().mq_combine_experts_to(Y.data_ptr(), _DT[Y.dtype], ldy, S, C, slots.data_ptr(), weights.data_ptr(), T, k,
+                                               out.data_ptr(), _DT[out_dtype], C, _stream(Y))
+    check(rc, "mq_combine_experts_to")
     return out
 
 

@@ -3,8 +3,8 @@
 import pytest
 import torch
 
-from moe_quant_amd import ops
-from test_gpu_routing_int8 import DT, _check_route, _gen, _say
+from moe_quant_amd import moe_layer, ops
+from test_gpu_routing_int8 import DT, U, _check_route, _experts, _gen, _half, _product64, _say
 
 pytestmark = pytest.mark.gpu
 
@@ -72,3 +72,48 @@ def test_all_chosen_from_a_coarse_grid(dev, score, E, k):
     for kw in (dict(), dict(bias=torch.zeros(E, device=dev)), dict(renormalize=False, scale=2.5)):
         w, i = _check_route(dev, l, k, score=score, **kw)
         assert all(len(set(r)) == k for r in i.tolist())
+
+
+# ---- the experts' weighted sum ----------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("S,C,T,k", [(1, 1, 1, 1), (16, 7168, 2, 8), (100, 33, 25, 4), (64, 2048, 64, 1), (30, 1000, 10, 3),
+                                     (50, 2056, 7, 9), (5, 64, 0, 2), (0, 64, 3, 2)])
+def test_combine_rounds_fp32_outputs_once(dev, dtype, S, C, T, k):
+    dt, g = DT[dtype], _gen(S * C + T)
+    Y = torch.randn(S, C, generator=g)
+    slots = torch.randint(0, max(S, 1), (T, k), generator=g, dtype=torch.int32)
+    if T > 2:
+        slots[1, 0], slots[2], slots[0, -1] = -1, -1, S
+    w = torch.rand(T, k, generator=g) - 0.3
+    live = ((slots >= 0) & (slots < S)).double()[..., None]
+    terms = (Y.double()[slots.clamp(0, S - 1).long()] if S else torch.zeros(T, k, C, dtype=torch.float64)) * w.double()[..., None] * live
+    want, mag = terms.sum(1), terms.abs().sum(1)
+    tol = k * U * mag * (1 + _half(dt)) + _half(dt) * want.abs() + (2.0**-25 if dt == torch.float16 else 2.0**-140)
+    for view in (Y.to(dev), torch.cat([Y, Y], 1).to(dev)[:, :C], torch.cat([Y[:, :1], Y], 1).to(dev)[:, 1:]):
+        out = ops.combine_experts(view, slots.to(dev), w.to(dev), dt)
+        assert out.dtype == dt and out.shape == (T, C) and ((out.cpu().double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("T,E,k,C,I", [(4, 16, 8, 256, 64), (64, 24, 8, 512, 128), (700, 8, 4, 264, 96), (5000, 6, 2, 128, 64)])
+def test_experts_outputs_are_rounded_after_their_sum(dev, dtype, T, E, k, C, I):
+    """The last two stages against 64 bits on what the two before gave.  The outputs of a token's experts are of both signs, so
+    their sum is smaller than they are: a rounding of each one to the tokens' type would be off by half a step of the terms,
+    not of the sum.  Roundings: five in 32 bits for a product, one for each term and its addition, one for the result."""
+    dt, g = DT[dtype], _gen(T + E)
+    x = torch.randn(T, C, generator=g).to(dt).to(dev)
+    ex = _experts(g, E, C, I, dev)
+    ids = torch.stack([torch.randperm(E, generator=g)[:k] for _ in range(T)]).to(dev)
+    weights = (torch.rand(T, k, generator=g) + 0.1).to(dev)
+    y = moe_layer.experts_forward_int8(x, ids, weights, ex)
+    rows, offsets, slots = ops.sort_by_expert(ids, E)
+    h = ops.matmul_int8_grouped(*ops.quantize_tokens(x), ex.gate_up, ex.gate_up_scale, offsets, rows, dt, True)
+    q, s = (t.cpu() for t in ops.quantize_tokens(h))
+    each = torch.empty(T * k, C, dtype=torch.float64)
+    for e in range(E):
+        lo, hi = offsets[e].item(), offsets[e + 1].item()
+        each[lo:hi] = _product64(q[lo:hi], s[lo:hi], ex.down[e].cpu(), ex.down_scale[e].cpu())[0]
+    terms = each[slots.long().cpu()] * weights.cpu().double()[..., None]
+    want, mag = terms.sum(1), terms.abs().sum(1)
+    tol = (6 + k) * U * mag * 1.01 + _half(dt) * want.abs() + (2.0**-25 if dt == torch.float16 else 2.0**-140)
+    assert y.dtype == dt and ((y.cpu().double() - want).abs() <= tol).all()

@@ -1,0 +1,27 @@
+"""Routing and 8-bit products without a GPU: refusals beyond those of test_routing_int8_host."""
+import ctypes
+
+import pytest
+import torch
+
+from moe_quant_amd import _lib, ops
+
+F32, BF16, F16, I32 = torch.float32, torch.bfloat16, torch.float16, torch.int32
+
+
+def test_combine_types():
+    s, w = torch.zeros(3, 2, dtype=I32), torch.zeros(3, 2)
+    for y, to in ((BF16, F32), (BF16, F16), (F16, BF16), (F16, F32), (F32, torch.float64), (F32, torch.int8)):
+        with pytest.raises(ValueError):
+            ops.combine_experts(torch.zeros(4, 8, dtype=y), s, w, to)
+    for y, to in ((BF16, BF16), (F16, F16), (F32, F32), (F32, BF16), (F32, F16), (BF16, None)):
+        with pytest.raises(_lib.MoeQuantHipError):  # fine but for the device
+            ops.combine_experts(torch.zeros(4, 8, dtype=y), s, w, to)
+    lib = _lib.load()
+    p = ctypes.cast(ctypes.create_string_buffer(64), ctypes.c_void_p)
+    f32, bf16, f16 = _lib.DT_F32, _lib.DT_BF16, _lib.DT_F16
+    for y, to in ((bf16, f32), (bf16, f16), (f16, bf16), (f16, f32), (f32, 3), (f32, -1), (3, 3)):
+        assert lib.mq_combine_experts_to(p, y, 8, 2, 8, p, p, 2, 2, p, to, 8, None) == _lib.MQ_ERR_ARG
+    for y, to in ((bf16, bf16), (f32, bf16), (f32, f16), (f32, f32)):
+        assert lib.mq_combine_experts_to(p, y, 8, 2, 8, p, p, 0, 2, p, to, 8, None) == _lib.MQ_OK
+        assert lib.mq_combine_experts_to(p, y, 8, 2, 8, p, p, 2, 2, p, to, 7, None) == _lib.MQ_ERR_ARG
