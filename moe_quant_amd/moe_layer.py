@@ -45,8 +45,10 @@ class LayerResult:
 
 def route_tokens(expert_ids: torch.Tensor, n_experts: int):
     """expert_ids (T, top_k) -> (order, offsets): order[offsets[e]:offsets[e+1]] are the token rows of expert e."""
-    # (what the sort's 32-bit positions cannot hold goes the other way)
-    if expert_ids.is_cuda and expert_ids.dtype == torch.int64 and n_experts <= 1024 and expert_ids.numel() < (1 << 31) - 8192:
+    # (what the sort does not take goes the other way: other types and shapes, no choices at all, no experts or too many, more
+    # choices than its 32-bit positions hold)
+    if (expert_ids.is_cuda and expert_ids.dtype == torch.int64 and expert_ids.dim() == 2 and expert_ids.shape[1] >= 1
+            and 1 <= n_experts <= 1024 and expert_ids.numel() < (1 << 31) - 8192):
         rows, offsets, _ = ops.sort_by_expert(expert_ids, n_experts)
         offsets = offsets.tolist()
         if offsets[-1] != rows.numel():

@@ -117,3 +117,14 @@ def test_experts_outputs_are_rounded_after_their_sum(dev, dtype, T, E, k, C, I):
     want, mag = terms.sum(1), terms.abs().sum(1)
     tol = (6 + k) * U * mag * 1.01 + _half(dt) * want.abs() + (2.0**-25 if dt == torch.float16 else 2.0**-140)
     assert y.dtype == dt and ((y.cpu().double() - want).abs() <= tol).all()
+
+
+# ---- ids that the layer driver's own sort does not take ------------------------------------------------------------
+@pytest.mark.parametrize("shape,E", [((5, 0), 4), ((0, 3), 4), ((0, 3), 0), ((0, 0), 2), ((2, 3, 1), 4), ((7, 2), 1025)])
+def test_route_tokens_of_any_shape_matches_the_host(dev, shape, E):
+    ids = torch.zeros(shape, dtype=torch.int64)
+    if ids.dim() == 3:
+        ids[1] = 3
+    want_rows, want = moe_layer.route_tokens(ids, E)
+    rows, offsets = moe_layer.route_tokens(ids.to(dev), E)
+    assert rows.dtype == torch.int64 and torch.equal(rows.cpu(), want_rows) and offsets == want
