@@ -545,6 +545,10 @@ __global__ __launch_bounds__(64 * Tile<BM>::WAVES) __attribute__((amdgpu_waves_p
 template <int DT, bool SWIGLU, int BM>
 int tile_launch(const Int8Args& a, hipStream_t st) {
   typedef Tile<BM> T;
+  const int outn = SWIGLU ? T::BN / 2 : T::BN, nt = (a.N + outn - 1) / outn;
+  // The kernel counts tiles in 32 bits, and offsets come from the device: were every expert's range all rows, the counts
+  // would still have to fit (the table of starts ascends only then).
+  if ((long)a.E * (a.M / BM + 1) * nt > 0x7fff0000L) return MQ_ERR_TOO_LARGE;  // (65535 spare, for steps of a whole grid)
   static std::atomic<int> cus[64];  // per GPU: its CUs, once the kernel may take its shared memory there
   int dev = -1;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return MQ_ERR_LAUNCH;
@@ -558,9 +562,7 @@ int tile_launch(const Int8Args& a, hipStream_t st) {
     cus[dev].store(n);
   }
   const long mt = a.offsets ? (long)a.M / BM + min(a.E, a.M) : ((long)a.M + BM - 1) / BM;
-  const int outn = SWIGLU ? T::BN / 2 : T::BN;
-  const long jobs = mt * ((a.N + outn - 1) / outn);
-  if (jobs > 0x7fffffffL) return MQ_ERR_TOO_LARGE;
+  const long jobs = mt * nt;
   const int grid = (int)min((long)n * T::PER_CU, (jobs + 7) / 8 * 8);
   hipLaunchKernelGGL((int8_tile_kernel<DT, SWIGLU, BM>), dim3(grid), dim3(64 * T::WAVES), sizeof(TileShared<BM>), st, a);
   return mq_check_launch();

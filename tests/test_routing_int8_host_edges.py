@@ -25,3 +25,17 @@ def test_combine_types():
     for y, to in ((bf16, bf16), (f32, bf16), (f32, f16), (f32, f32)):
         assert lib.mq_combine_experts_to(p, y, 8, 2, 8, p, p, 0, 2, p, to, 8, None) == _lib.MQ_OK
         assert lib.mq_combine_experts_to(p, y, 8, 2, 8, p, p, 2, 2, p, to, 7, None) == _lib.MQ_ERR_ARG
+
+
+def test_grouped_tiles_beyond_32_bits_are_refused():
+    """Offsets come from the device and may say that every expert has all rows: where the kernel could not count such tiles in 32
+    bits, the call is refused before a device is looked for."""
+    lib = _lib.load()
+    p = ctypes.cast(ctypes.create_string_buffer(64), ctypes.c_void_p)
+
+    def grouped(S, E, N, swiglu=0, K=32):
+        return lib.mq_matmul_int8_grouped(p, K, p, 4, p, S, p, K, N * K * (1 + swiglu), p, E, p, p, N, 1, N, K, swiglu, None)
+
+    assert grouped(1 << 30, 1024, 8) == _lib.MQ_ERR_TOO_LARGE
+    assert grouped(1 << 24, 1024, 16384) == _lib.MQ_ERR_TOO_LARGE
+    assert grouped(1 << 24, 1024, 7168, 1) == _lib.MQ_ERR_TOO_LARGE
