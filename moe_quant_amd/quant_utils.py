@@ -129,7 +129,8 @@ def linear_int8(x: Tensor, weight: Tensor, weight_scale: Tensor, bias: Optional[
         raise ValueError("x must be (..., C)")
     if x.dim() == 2:
         return ops.linear_int8(x, weight, weight_scale, bias)
-    return ops.linear_int8(x.reshape(-1, x.shape[-1]), weight, weight_scale, bias).view(*x.shape[:-1], weight.shape[0])
+    tokens = x.reshape(x.shape[:-1].numel(), x.shape[-1])  # (-1 has no meaning where there are no columns)
+    return ops.linear_int8(tokens, weight, weight_scale, bias).view(*x.shape[:-1], weight.shape[0])
 
 
 def get_relative_mse_error(q: Tensor, w: Tensor, H: Optional[Tensor] = None):

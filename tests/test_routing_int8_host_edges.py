@@ -4,7 +4,7 @@ import ctypes
 import pytest
 import torch
 
-from moe_quant_amd import _lib, ops
+from moe_quant_amd import _lib, ops, quant_utils
 
 F32, BF16, F16, I32 = torch.float32, torch.bfloat16, torch.float16, torch.int32
 
@@ -39,3 +39,11 @@ def test_grouped_tiles_beyond_32_bits_are_refused():
     assert grouped(1 << 30, 1024, 8) == _lib.MQ_ERR_TOO_LARGE
     assert grouped(1 << 24, 1024, 16384) == _lib.MQ_ERR_TOO_LARGE
     assert grouped(1 << 24, 1024, 7168, 1) == _lib.MQ_ERR_TOO_LARGE
+
+
+def test_linear_without_columns_is_refused_in_any_shape():
+    for x in (torch.zeros(0), torch.zeros(2, 0), torch.zeros(2, 3, 0), torch.zeros(0, 3, 0)):
+        with pytest.raises(ValueError):
+            quant_utils.linear_int8(x, torch.zeros(6, 0, dtype=torch.int8), torch.zeros(6))
+    with pytest.raises(_lib.MoeQuantHipError):  # no tokens, but columns: fine but for the device
+        quant_utils.linear_int8(torch.zeros(0, 3, 32), torch.zeros(6, 32, dtype=torch.int8), torch.zeros(6))
