@@ -105,6 +105,8 @@ class Int8Experts:
         gu, gus, dn, dns = [], [], [], []
         for gate, up, down in experts:
             (g, gs), (u, us), (d, ds) = (quant_utils.int8_weight(*w) for w in (gate, up, down))
+            if g.shape != u.shape or d.shape != g.shape[::-1]:
+                raise ValueError("an expert's gate and up must be (I, C) and its down (C, I)")
             gu.append(torch.cat([g, u]))
             gus.append(torch.cat([gs, us]))
             dn.append(d)

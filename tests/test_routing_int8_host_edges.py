@@ -4,7 +4,7 @@ import ctypes
 import pytest
 import torch
 
-from moe_quant_amd import _lib, ops, quant_utils
+from moe_quant_amd import _lib, moe_layer, ops, quant_utils
 
 F32, BF16, F16, I32 = torch.float32, torch.bfloat16, torch.float16, torch.int32
 
@@ -47,3 +47,13 @@ def test_linear_without_columns_is_refused_in_any_shape():
             quant_utils.linear_int8(x, torch.zeros(6, 0, dtype=torch.int8), torch.zeros(6))
     with pytest.raises(_lib.MoeQuantHipError):  # no tokens, but columns: fine but for the device
         quant_utils.linear_int8(torch.zeros(0, 3, 32), torch.zeros(6, 32, dtype=torch.int8), torch.zeros(6))
+
+
+def test_experts_whose_halves_differ_are_refused():
+    """Gate and up rows are stacked: with six and two of them the products would pair the wrong ones."""
+    mk = lambda r, c: (torch.full((r, c), 8, dtype=torch.uint8), torch.ones(r, 1), torch.full((r, 1), 8.0))
+    from_quantized = moe_layer.Int8Experts.from_quantized
+    assert from_quantized([(mk(4, 8), mk(4, 8), mk(8, 4))]).gate_up.shape == (1, 8, 8)
+    for bad in ((mk(6, 8), mk(2, 8), mk(8, 4)), (mk(4, 8), mk(4, 6), mk(8, 4)), (mk(4, 8), mk(4, 8), mk(8, 6)), (mk(4, 8), mk(4, 8), mk(6, 4))):
+        with pytest.raises(ValueError):
+            from_quantized([bad])
