@@ -114,14 +114,20 @@ class Int8Experts:
         return cls(torch.stack(gu), torch.stack(gus), torch.stack(dn), torch.stack(dns))
 
 
+# values of the experts' fp32 outputs that are alive at a time (16 GiB): more tokens than that go in equal parts, one after the
+# other, with the same results.  A part of 74898 tokens of eight experts of 7168 reads its 11 GB of weights in a twentieth of
+# the time it takes in all.
+_OUTPUTS_AT_ONCE = 1 << 32
+
+
 @torch.no_grad()
 def experts_forward_int8(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, experts: Int8Experts) -> torch.Tensor:
     """The expert part of a block's forward on its quantized weights:
     y[t] = sum_j weights[t, j] * down_e(silu(gate_e(x[t])) * up_e(x[t])), e = ids[t, j].  x (T, C) fp32, bf16 or fp16; ids
     (T, top_k) int64 and weights (T, top_k) fp32 as a `Router` gives them (ids outside the experts add nothing).  Tokens and
     the product between the projections, held in x's type, are quantized to 8 bits with a scale per row; the experts' outputs
-    are fp32 (T * top_k * C values of scratch memory) and rounded once, after their weighted sum.  Nothing is read back to
-    the host."""
+    are fp32 and rounded once, after their weighted sum (scratch memory for T * top_k * C values, at most 2^32 of them at a
+    time).  Nothing is read back to the host."""
     if experts.gate_up.dim() != 3 or experts.down.dim() != 3:
         raise ValueError("gate_up must be (E, 2 I, C) and down (E, C, I)")
     E, C = experts.gate_up.shape[0], experts.gate_up.shape[2]
@@ -129,6 +135,15 @@ def experts_forward_int8(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tens
         raise ValueError("x must be (T, C) with the experts' C, ids and weights (T, top_k)")
     if experts.gate_up.shape[1] % 2 or experts.down.shape != (E, C, experts.gate_up.shape[1] // 2):
         raise ValueError("gate_up must be (E, 2 I, C) and down (E, C, I)")
+    T = x.shape[0]
+    parts = -(-T // max(1, _OUTPUTS_AT_ONCE // max(1, ids.shape[1] * C)))
+    if parts > 1:
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        step = -(-T // parts)
+        for t in range(0, T, step):
+            part = slice(t, t + step)
+            out[part] = experts_forward_int8(x[part], ids[part], weights[part], experts)
+        return out
     rows, offsets, slots = ops.sort_by_expert(ids, E)
     codes, scale = ops.quantize_tokens(x)
     h = ops.matmul_int8_grouped(codes, scale, experts.gate_up, experts.gate_up_scale, offsets, rows, x.dtype, swiglu=True)

@@ -128,3 +128,41 @@ def test_route_tokens_of_any_shape_matches_the_host(dev, shape, E):
     want_rows, want = moe_layer.route_tokens(ids, E)
     rows, offsets = moe_layer.route_tokens(ids.to(dev), E)
     assert rows.dtype == torch.int64 and torch.equal(rows.cpu(), want_rows) and offsets == want
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_experts_of_many_tokens_go_in_parts(dev, dtype, monkeypatch):
+    """With the bound on the experts' fp32 outputs brought down: the same bits, and no more scratch memory than it allows."""
+    dt, g = DT[dtype], _gen(40)
+    T, E, k, C, I = 5001, 12, 4, 512, 64
+    x = torch.randn(T, C, generator=g).to(dt).to(dev)
+    ex = _experts(g, E, C, I, dev)
+    ids = torch.stack([torch.randperm(E, generator=g)[:k] for _ in range(T)]).to(dev)
+    ids[7, 1], ids[4000] = -1, E
+    weights = torch.rand(T, k, generator=g).to(dev)
+
+    def peak(limit):
+        monkeypatch.setattr(moe_layer, "_OUTPUTS_AT_ONCE", limit)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        y = moe_layer.experts_forward_int8(x, ids, weights, ex)
+        torch.cuda.synchronize()
+        return y, torch.cuda.max_memory_allocated() - before
+
+    whole, much = peak(1 << 32)
+    assert much >= 4 * T * k * C
+    for limit in (T * k * C - 1, 1 << 21, 1 << 20, k * C, 1):
+        if limit < 1 << 18:  # a token at a time: a few of them
+            monkeypatch.setattr(moe_layer, "_OUTPUTS_AT_ONCE", limit)
+            assert torch.equal(moe_layer.experts_forward_int8(x[:9], ids[:9], weights[:9], ex), whole[:9])
+            continue
+        y, little = peak(limit)
+        assert torch.equal(y, whole) and y.is_contiguous()
+        # the result, a part of it, and the part's outputs; its codes, activations and places are a quarter of those
+        assert little <= 2 * y.nbytes + 1.25 * 4 * limit + (1 << 20)
+    strided = torch.randn(C, T, generator=g).to(dt).to(dev).t()
+    monkeypatch.setattr(moe_layer, "_OUTPUTS_AT_ONCE", 1 << 20)
+    y = moe_layer.experts_forward_int8(strided, ids, weights, ex)
+    monkeypatch.setattr(moe_layer, "_OUTPUTS_AT_ONCE", 1 << 32)
+    assert torch.equal(y, moe_layer.experts_forward_int8(strided, ids, weights, ex))
