@@ -10,7 +10,8 @@ namespace {
 // TPR threads per token, eight values each in turn: the largest magnitude first, then the codes, from the NV vectors a
 // thread keeps in registers (NV = 0: rows too long for that, read twice, the second time from the cache).  A row that holds
 // a NaN or an infinity gets scale NaN and codes 0: its products are NaN, no other token's are.
-// Bound by memory: 176 us for 16384 x 16384 bf16 (4.6 TB/s read and written; read twice and element by element it took 587).
+// Bound by memory: 163 to 180 us for 16384 x 16384 bf16 (4.5 to 4.9 TB/s read and written; read twice and element by element it
+// took 587); 7 us for 333 x 7168.
 template <int DT, int TPR, int NV>
 __global__ __launch_bounds__(256) void quantize_tokens_kernel(const void* __restrict__ X, long ldx, int n, int C,
                                                               int8_t* __restrict__ Q, long ldq, float* __restrict__ scale) {
@@ -118,8 +119,10 @@ __global__ __launch_bounds__(256) void align_rows_kernel(const int8_t* __restric
 }
 
 size_t padded(int K) { return ((size_t)K + 15) / 16 * 16; }
-// K no multiple of 4: contiguous rows start anywhere; large products copy them first (30 us for 8192 x 7781 weights against
-// the millisecond that such rows cost a product of 4096 tokens)
+// K no multiple of 4: contiguous rows start anywhere; large plain products copy them first (at 4096 x 8192 x 7781 the copies
+// take 24 + 13 us and the product 250, on the rows as they are 2460).  Rows off the alignment with K a multiple of 4 are views,
+// which are never copied (713 us at 4096 x 4096 x 4096 where aligned rows take 70), nor are the rows of grouped products (3600
+// us for 16384 rows over 64 experts of 2048 x 4095 where 2048 x 4096 takes 180).
 bool aligns_rows(int M, int N, int K, int swiglu) { return K % 4 != 0 && K >= 16 && small_tiles(M, N, swiglu); }
 
 int int8_dispatch(Int8Args a, int dtype, int swiglu, int8_t* ws, hipStream_t st) {

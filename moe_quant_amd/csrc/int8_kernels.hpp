@@ -156,9 +156,9 @@ __device__ __forceinline__ intx4 short_row(const int8_t* row, int k, int K, bool
 //   The end of a row: a chunk that reaches beyond K is loaded from the last 16 bytes of the row instead (never outside it),
 //   and the tokens' fragments drop the bytes that belong to earlier chunks, or all of them.
 //   A wavefront computes only the 32-row blocks (NB of its four or two) that hold any rows.
-// Measured: 481 us at 8192 x 8192 x 8192 (2.29 POP/s), 1.6 to 1.8 ms at 16384 x 7168 x 16384 (2.1 to 2.4; the clock falls to
-// 1.6 GHz there, so power decides); large library products of 8-bit integers reach 2.1 to 2.6.  Grouped, 32 rows for each of
-// 128 experts of 4096 x 7168: 646 us, 5.8 TB/s of weights.  Tried: four stages of 64 bytes instead of two of 128 (5% slower
+// Measured: 476 to 571 us at 8192 x 8192 x 8192 (1.9 to 2.3 POP/s), 1.53 to 1.75 ms at 16384 x 7168 x 16384 (2.2 to 2.5; the
+// clock falls to 1.6 GHz there, so power decides); large library products of 8-bit integers reach 2.1 to 2.6.  Grouped, 32
+// rows for each of 128 experts of 4096 x 7168: 643 us, 5.8 TB/s of weights.  Tried: four stages of 64 bytes instead of two of 128 (5% slower
 // on large products: memory serves 64-byte requests), tiles of 128 x 256 (15% slower: half again as many loads).
 constexpr int TK = 128, NST = 2;
 constexpr int MIN_STAGES = 3;  // what the hand-over to the next tile needs; beyond K everything counts as zero
@@ -575,8 +575,9 @@ int tile_launch(const Int8Args& a, hipStream_t st) {
 //   loaded like that, an instruction touches every row four times and the address unit takes 64 cycles for it.)  Chunk c of
 //   row r lies at position c ^ (r / 4 % 4): 16 lanes reading chunk c of 16 rows touch every bank once.
 //   D = 0: fragments straight from memory, UN steps at a time; any alignment, any K.
-// Measured: 12 us at 333 x 576 x 7168 (D = 0: 16), 6.5 at 8 x 2048 x 7168 (8.6); bound by the way of the operands to the
-// wavefronts, or by the weights' bytes: 41 us at 16 x 18432 x 7168 (3.3 TB/s).
+// Measured, on weights that no cache holds: 12 us at 333 x 576 x 7168 (D = 0: 16), 6.8 at 8 x 2048 x 7168 (D = 0: 11); bound by
+// the way of the operands to the wavefronts (D = 2 has a single step in flight, which it waits for in full), or by the
+// weights' bytes: 41 us at 16 x 18432 x 7168 (3.2 TB/s).
 constexpr int vmcnt_is(int n) { return 0x0070 | (n & 15) | (n >> 4) << 14; }  // ... and lgkmcnt(0)
 
 template <int DT, bool SWIGLU, int R, int C, int UN, int D>
@@ -786,7 +787,8 @@ int thin_launch(const Int8Args& a, hipStream_t st) {
 // itself (XDT = their type), under the first weights' way from memory.  Any alignment; K of at least 16.
 //   A row's last chunk, where K is no multiple of 16, is its last 16 bytes, and the tokens' bytes that belong to the chunk
 //   before are zero there.
-// Measured: one token, quantized on the way, 7.2 us at 2048 x 7168; 26 us at 18432 x 7168 (5.1 TB/s).
+// Measured: one token, quantized on the way, 8.5 us at 2048 x 7168 (6.7 on weights that a cache holds), 28.5 at 18432 x 7168
+// (4.6 TB/s).
 constexpr int VT = 2, VEC_THREADS = 256, VEC_CHUNKS = 8;
 
 template <int DT, bool SWIGLU, int XDT>
@@ -977,8 +979,8 @@ int vector_launch(const Int8Args& a, hipStream_t st) {
     set.fetch_or(1ull << dev);
   }
   const int pairs = SWIGLU ? a.N : (a.N + 1) / 2, waves = VEC_THREADS / 64;
-  // 512 workgroups, two a CU, walk over what they do not reach at once: 26 us at 18432 x 7168 (5.1 TB/s) against 32 with 256
-  // of them and 30 with 2048; 6.3 us at 2048 x 7168 (256 workgroups)
+  // 512 workgroups, two a CU, walk over what they do not reach at once: 28.5 us at 18432 x 7168 against 35 with 256 of them and
+  // 39 with 2048 (2048 x 7168 has 256)
   const int gx = min((pairs + waves - 1) / waves, 512);
   hipLaunchKernelGGL((int8_vector_kernel<DT, SWIGLU, XDT>), dim3(gx), dim3(VEC_THREADS),
                      vector_smem(a.K), st, a);
@@ -1004,20 +1006,22 @@ template <int DT, bool SWIGLU>
 int int8_launch(const Int8Args& a, hipStream_t st) {
   const bool tiles = a.K >= 16 && rows_of_words(a.A, a.lda) && rows_of_words(a.B, a.ldb) && a.strideB % 4 == 0;
   if (a.offsets) {
-    // A decode step: 110 + 71 us without shared memory against 139 + 70 with tiles at 32 rows over 64 experts of 7168 x 2048,
-    // 201 + 125 against 205 + 125 at 128 rows; at 512 rows the tiles win, 296 + 195 against 388 + 217.
-    // (Staging the rows costs there: 130 + 78.)
+    // A decode step: gate/up + down of 64 experts of 7168 x 2048, skewed loads, us without shared memory against tiles: 32
+    // rows 100 + 65 against 133 + 51, 64 rows 126 + 87 against 143 + 73, 128 rows 171 + 114 against 156 + 99, 256 rows 229 +
+    // 145 against 221 + 122, 512 rows 322 + 191 against 237 + 148 (even loads alike).  So the border lies nearer to one row an
+    // expert than to the four below, for the down product lower still.  (Staging the rows costs at 32 rows: 130 + 78 where
+    // 110 + 71 was measured beside it.)
     if (!tiles || a.M <= 4l * a.E) return thin_launch<DT, SWIGLU, 2, 2, 2, 0>(a, st);
     // Few rows an expert: the weights' bytes decide, and two small workgroups a CU keep more of them in flight (5.8 against
     // 4.9 TB/s at 32 rows for each of 128 experts of 7168 x 2048).  Many rows: large tiles read both operands less often
-    // (1830 against 1480 TOP/s at 256 rows), if there are enough of them to go round several times.
+    // (1850 against 1510 TOP/s at 256 rows), if there are enough of them to go round several times.
     if (a.M <= 128l * a.E || !enough_jobs<SWIGLU>(a)) return tile_launch<DT, SWIGLU, 128>(a, st);
     return tile_launch<DT, SWIGLU, 256>(a, st);
   }
   if (for_vector(a.M, a.K)) return vector_launch<DT, SWIGLU, -1>(a, st);
-  // 76 us at 4096 x 4096 x 4096 (256 large tiles) against 103 with small ones; 57 against 48 at 2048 x 4096 x 4096 (128)
+  // 70 us at 4096 x 4096 x 4096 (256 large tiles) against 97 with small ones; 66 against 51 at 2048 x 4096 x 4096 (128)
   if (tiles && enough_tiles(a.M, a.N, SWIGLU, 256, 192)) return tile_launch<DT, SWIGLU, 256>(a, st);
-  // 62 us at 128 x 18432 x 7168 (144 small tiles) against 80 without tiles; 34 against 30 at 512 x 4096 x 4096 (128)
+  // 64 us at 128 x 18432 x 7168 (144 small tiles) against 80 without tiles; 28 against 29 at 512 x 4096 x 4096 (128)
   if (tiles && small_tiles(a.M, a.N, SWIGLU)) return tile_launch<DT, SWIGLU, 128>(a, st);
   // the largest block of results that still gives 192 workgroups (and is half full, at least)
   const auto groups = [&](int R, int C) {
@@ -1030,10 +1034,10 @@ int int8_launch(const Int8Args& a, hipStream_t st) {
     return thin_launch<DT, SWIGLU, 1, 2, 2, 0>(a, st);
   }
   if (groups(4, 4) >= 192) return thin_launch<DT, SWIGLU, 4, 4, 1, 2>(a, st);  // 11 us at 512 x 2048 x 2048, (2, 4) 14, (2, 2) 15
-  if (groups(2, 4) >= 192) return thin_launch<DT, SWIGLU, 2, 4, 1, 2>(a, st);  // 23 us at 64 x 7168 x 7168, (4, 4) 32, (2, 2) 27
-  if (groups(2, 2) >= 192) return thin_launch<DT, SWIGLU, 2, 2, 1, 2>(a, st);  // 12 us at 333 x 576 x 7168, (2, 4) 17, (1, 1) 16
-  if (groups(1, 2) >= 192 || SWIGLU) return thin_launch<DT, SWIGLU, 1, 2, 1, 3>(a, st);  // 4.8 us at 64 x 2048 x 2048, (1, 1) 5.8
-  return thin_launch<DT, SWIGLU, 1, SWIGLU ? 2 : 1, 1, 4>(a, st);  // 6.5 us at 8 x 2048 x 7168, (1, 2) 8.7
+  if (groups(2, 4) >= 192) return thin_launch<DT, SWIGLU, 2, 4, 1, 2>(a, st);  // 22 us at 64 x 7168 x 7168, (4, 4) 32, (2, 2) 26
+  if (groups(2, 2) >= 192) return thin_launch<DT, SWIGLU, 2, 2, 1, 2>(a, st);  // 12 us at 333 x 576 x 7168, (2, 4) 16, (1, 1) 16
+  if (groups(1, 2) >= 192 || SWIGLU) return thin_launch<DT, SWIGLU, 1, 2, 1, 3>(a, st);  // 5.4 us at 64 x 2048 x 2048, (1, 1) 6.0
+  return thin_launch<DT, SWIGLU, 1, SWIGLU ? 2 : 1, 1, 4>(a, st);  // 6.8 us at 8 x 2048 x 7168, (1, 2) 8.7
 }
 
 }  // namespace

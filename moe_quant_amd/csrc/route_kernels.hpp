@@ -184,8 +184,9 @@ __global__ __launch_bounds__(256) void route_exact_kernel(RouteArgs a) {
 //   belong to the k best (scores down to the k-th less the error) is ranked again by its exact 64-bit score; more than 16 of
 //   them, or infinite logits, send the row the exact way.  Groups too close at the border of the choice: by their exact scores.
 // At 256 experts about 650 vector instructions for four rows (63 comparators of the sort, 16 exponentials, 9 rounds of 4 + 2
-// + shifts); reading 4 KB takes about as long.  Measured: 248 us for 1048576 x 256 fp32 logits (4.7 TB/s; the exact way alone
-// 2700), 36 to 38 for 65536 rows with groups and bias (bound by instructions), 5.5 for one row.
+// + shifts); reading 4 KB takes about as long.  Measured: 251 us for 1048576 x 256 fp32 logits (4.7 TB/s; the exact way alone
+// 3800), 36 to 38 for 65536 rows with groups and bias (bound by instructions), 5.3 for one row.  17 choices and more go the
+// exact way: 420 us for 65536 x 256 where 16 choices take 43.
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);

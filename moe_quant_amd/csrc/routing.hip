@@ -14,9 +14,10 @@ constexpr int ROUTE_MAX_E = 1024;
 // ---- sort by expert -----------------------------------------------------------------------------------
 // Stable counting sort of n = T * top_k choices into E + 1 bins (bin E: ids outside [0, E)).  A workgroup owns a run of
 // SORT_CHUNK choices; `count` holds, bin-major, the number of choices of every (bin, workgroup).
-// Measured: 144 us for 16.8 million choices over 256 experts (35 counting, 7 summing, 102 placing: 3.3 TB/s of its bytes), 5 us
-// for 488 in one workgroup.  Tried: chunks of 4096 and 16384 (108 and 120 us placing); putting a workgroup's choices in order
-// in shared memory first, so that rows leaves in runs (121).
+// Measured: 146 us of kernels for 16.8 million choices over 256 experts of skewed loads (34 counting, 7 summing, 105 placing;
+// 166 us a pass, with the gaps between three launches; even loads take 170 placing), 5 us for 488 in one workgroup.  Tried, at
+// 102 placing: chunks of 4096 and 16384 (108 and 120); putting a workgroup's choices in order in shared memory first, so that
+// rows leaves in runs (121).
 constexpr int SORT_CHUNK = 8192;
 constexpr int SORT_WAVES = 8;
 constexpr int SORT_MAX_E = 1024;
@@ -164,8 +165,8 @@ __global__ __launch_bounds__(512) void sort_scatter_kernel(const long* __restric
 
 // ---- combine --------------------------------------------------------------------------------------------
 // One workgroup per (token, 2048 columns); the sum runs in the order of the token's choices, in 32 bits, and is rounded
-// once, to the type TO of the results.  Slots outside [0, S) add nothing.  Bound by memory: 220 us for 8192 tokens of eight
-// experts, 7168 bf16 columns (4.8 TB/s).
+// once, to the type TO of the results.  Slots outside [0, S) add nothing.  Bound by memory, for 8192 tokens of eight experts of
+// 7168 columns: 397 us from fp32 to bf16 (5.0 TB/s), 223 from bf16 (4.7).
 template <int DT, int TO, bool VEC>
 __global__ __launch_bounds__(256) void combine_kernel(const void* __restrict__ Y, long ldy, int S, int C,
                                                       const int* __restrict__ slots, const float* __restrict__ weights, int k,
