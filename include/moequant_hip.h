@@ -375,8 +375,8 @@ int mq_linear_int8(const void* X, int dtype, long ldx, const int8_t* B, long ldb
  * to [0, S]) are products with B + e * strideB, b_scale + e * N (swiglu: e * 2 N).  Row m of Y takes row rows[m] of A and
  * a_scale (rows : S int64 on the device; a value outside [0, src_rows) stands for a row of zeros) or, rows == NULL, row
  * m.  Rows of Y outside every range are left as they are; of rows in several ranges nothing is said.  E <= 1024.  src_rows
- * == 0: A and a_scale may be NULL.  MQ_ERR_TOO_LARGE where S rows for each of the E experts would be 2^31 tiles or more (of 128 x
- * 128 or 256 x 256; only matrices of more than a hundred gigabytes reach that, or more than 2^28 rows). */
+ * == 0: A and a_scale may be NULL.  MQ_ERR_TOO_LARGE where S rows for each of the E experts would be 2^31 - 65536 tiles of
+ * results or more, 128 x 64 the smallest: with 1024 experts only results beyond 30 GB or 2^28 rows reach that. */
 int mq_matmul_int8_grouped(const int8_t* A, long lda, const float* a_scale, int src_rows, const long* rows, int S,
                            const int8_t* B, long ldb, long strideB, const float* b_scale, int E, const long* offsets, void* Y,
                            long ldy, int out_dtype, int N, int K, int swiglu, void* stream);
